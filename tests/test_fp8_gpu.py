@@ -1,0 +1,258 @@
+"""8-bit rows, weights and products against the same in 64 bits: one row to many, odd sizes, slices of wider tensors, zeros,
+infinities, the borders of the scales; a run of them together as a feed-forward uses them; and captured runs."""
+import math
+
+import pytest
+import torch
+
+import fp8_util as fu
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from tiny_llm_b200 import ops
+    return ops
+
+
+def rng(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def randn(g, *shape):
+    return torch.randn(*shape, generator=g, device=DEV)
+
+
+def rows8(ops, x):
+    out = ops.fp8_rows(x.shape[0], x.shape[1], DEV)
+    ops.quantize_fp8(x, *out)
+    return out
+
+
+def weight8(ops, w):
+    out = ops.fp8_weight(w.shape[0], w.shape[1], DEV)
+    ops.quantize_weight_fp8(w, *out)
+    return out
+
+
+def same(got, want):
+    return bool(((got.double() == want) | (torch.isnan(got.double()) & torch.isnan(want))).all())
+
+
+def spread(g, m, k):
+    """Rows whose groups differ by many powers of two, with zeros among them."""
+    x = randn(g, m, k) * torch.exp2(torch.randint(-20, 20, (m, fu.groups(k)), generator=g, device=DEV).float()).repeat_interleave(128, 1)[:, :k]
+    x[torch.rand(m, k, generator=g, device=DEV) < 0.2] = 0
+    return x
+
+
+# ---------------------------------------------------------------------------------------------- rows and weights
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 128), (3, 127), (7, 129), (33, 2000), (5, 514), (300, 1030), (2, 14336), (1000, 136)])
+def test_rows_are_the_nearest_8_bit_values(ops, m, k, dtype):
+    g = rng(m * 31 + k)
+    wide = spread(g, m, k + 5).to(dtype)
+    for x in (wide[:, :k].contiguous(), wide[:, :k], wide[:, 5:]):
+        room = torch.full((m, -(-k // 16) * 16 + 16), 7, dtype=torch.uint8, device=DEV)
+        scales = torch.full((m, fu.groups(k) + 3), 7, dtype=torch.uint8, device=DEV)
+        out, sc = room.view(ops.FP8)[:, :k], scales.view(ops.FP8_SCALE)[:, : fu.groups(k)]
+        ops.quantize_fp8(x, out, sc)
+        want, ws = fu.quantize_rows(x)
+        assert same(out, want) and same(sc, ws)
+        assert bool((room[:, k:] == 7).all()) and bool((scales[:, fu.groups(k):] == 7).all())   # what lies behind stays
+
+
+def test_scales_at_their_borders(ops):
+    """Largest magnitudes at and next to 448 times powers of two, the smallest and largest floats, zeros, infinities, NaN."""
+    up = torch.tensor(448.0).nextafter(torch.tensor(1e9)).item()
+    edges = [448.0, up, 447.0, 1.75, 1.75 * 2.0 ** -100, 0.0, -0.0, 2.0 ** -149, 2.0 ** -126, 448 * 2.0 ** -126, up * 2.0 ** -126,
+             3.4028234663852886e38, -3.4028234663852886e38, math.inf, -math.inf, math.nan, 464.0, 1.0, 2.0 ** -10]
+    x = torch.zeros(len(edges), 300, device=DEV)
+    x[:, 1] = 2.0 ** -9 * 1.5                       # beside a 1 it is a tie between two 8-bit values or far below them
+    x[:, 290] = 1.0
+    for i, e in enumerate(edges):
+        x[i, 77] = e
+    out, sc = rows8(ops, x)
+    want, ws = fu.quantize_rows(x)
+    assert same(sc, ws) and same(out, want)
+    assert torch.isnan(sc.float()[13:16, 0]).all() and bool((out.float()[13:16, :128] == 0).all()) and bool((sc.float()[:, 2] == 2.0 ** -8).all())
+    blocks = torch.zeros(128 * len(edges), 130, device=DEV)
+    blocks[::128, 0] = x[:, 77]
+    data, scales = weight8(ops, blocks)
+    want, ws = fu.quantize_weight(blocks)
+    assert same(scales, ws) and same(data, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,k", [(1, 1), (127, 129), (128, 128), (300, 1000), (257, 4099), (2560, 2048)])
+def test_weights_are_the_nearest_8_bit_values(ops, n, k, dtype):
+    g = rng(n + k)
+    wide = (randn(g, n, k + 3) * torch.exp2(torch.randint(-9, 9, (n, 1), generator=g, device=DEV).float())).to(dtype)
+    for w in (wide[:, :k].contiguous(), wide[:, 3:]):
+        data, scales = weight8(ops, w)
+        want, ws = fu.quantize_weight(w)
+        assert same(data, want) and same(scales, ws)
+
+
+@pytest.mark.parametrize("m,k", [(1, 64), (3, 130), (8, 2048), (5, 4097), (40, 1000), (2, 20000), (700, 512)])
+def test_normed_rows(ops, m, k):
+    """The mean of squares and the two products in 32 bits: at most k / 512 + 20 roundings of 2^-24."""
+    g = rng(m + k)
+    x, w = spread(g, m + 2, k), 1 + 0.3 * randn(g, k)
+    x[m + 1] = 0
+    idx = torch.randperm(m + 2, generator=g, device=DEV)[: m + 1].to(torch.int32)
+    y = w.double() * x.double() / torch.sqrt((x.double() ** 2).mean(1, keepdim=True) + 1e-5)
+    off = y.abs() * (k / 512 + 20) * 2.0 ** -24
+    out = ops.fp8_rows(m + 2, k, DEV)
+    ops.rms_norm_fp8(x, w, 1e-5, *out)
+    assert fu.between_roundings(*out, y, off) and bool((out[0].float()[m + 1] == 0).all())
+    some = ops.fp8_rows(m + 1, k, DEV)
+    ops.rms_norm_fp8(x, w, 1e-5, *some, rows=idx)
+    assert torch.equal(some[0].view(torch.uint8), out[0].view(torch.uint8)[idx.long()]) and torch.equal(some[1].view(torch.uint8), out[1].view(torch.uint8)[idx.long()])
+
+
+# ---------------------------------------------------------------------------------------------- products
+
+
+SHAPES = [(1, 1, 1), (1, 2560, 2048), (2, 130, 300), (5, 1000, 129), (16, 64, 4096), (17, 4100, 520), (33, 700, 1152), (64, 512, 3584),
+          (65, 129, 700), (100, 4096, 640), (127, 300, 257), (128, 384, 128), (129, 128, 1000), (200, 1000, 1520), (257, 2000, 400),
+          (400, 5000, 384), (1000, 333, 260), (1500, 2304, 512), (2100, 4000, 200)]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_products_are_near_64_bits(ops, m, n, k):
+    g = rng(m + 3 * n + 7 * k)
+    a, w = rows8(ops, spread(g, m, k)), weight8(ops, randn(g, n, k))
+    w[1].mul_(torch.rand(w[1].shape, generator=g, device=DEV) + 0.5)        # scales of any value
+    want, off = fu.product(*a, *w)
+    full = torch.full((m, n + 5), 7.0, device=DEV)
+    for out in (torch.empty(m, n, device=DEV), full[:, :n], torch.full((m, n + 3), 7.0, device=DEV)[:, 3:]):
+        ops.linear_fp8(*a, *w, out)
+        assert bool(((out - want).abs() <= off + 2.0 ** -24 * want.abs()).all())
+    assert bool((full[:, n:] == 7.0).all())
+    short = torch.empty(m, n, dtype=torch.bfloat16, device=DEV)
+    ops.linear_fp8(*a, *w, short)
+    assert bool(((short.double() - want).abs() <= off + 2.0 ** -8 * (want.abs() + off)).all())
+    stream = randn(g, m, n)
+    acc = stream.clone()
+    ops.linear_fp8(*a, *w, acc, accumulate=True)
+    assert bool(((acc - (stream + want)).abs() <= off + 2.0 ** -24 * ((stream + want).abs() + want.abs() + off)).all())
+    again = torch.empty(m, n, device=DEV)
+    ops.linear_fp8(*a, *w, again)
+    assert torch.equal(again, full[:, :n])                                   # no order of sums changes from call to call
+    ops.check_status()
+
+
+@pytest.mark.parametrize("m", [3, 40, 150, 600])
+def test_rows_that_are_not_finite_spoil_no_other_row(ops, m):
+    g = rng(m)
+    n, k = 700, 1000
+    x = randn(g, m, k)
+    x[1, 5], x[2, 999] = math.inf, math.nan
+    a, w = rows8(ops, x), weight8(ops, randn(g, n, k))
+    out = torch.empty(m, n, device=DEV)
+    ops.linear_fp8(*a, *w, out)
+    clean = x.clone()
+    clean[1:3] = 0
+    want, off = fu.product(*rows8(ops, clean), *w)
+    assert bool(torch.isnan(out[1:3]).all())
+    keep = [i for i in range(m) if i not in (1, 2)]
+    assert bool(((out - want).abs() <= off + 2.0 ** -24 * want.abs())[keep].all())
+
+
+def gated_weight(ops, g, i, k):
+    blocks = fu.groups(i)
+    w = torch.zeros(2, blocks * 128, k, device=DEV)
+    w[:, :i] = randn(g, 2, i, k) / math.sqrt(k)
+    return weight8(ops, w.view(2, blocks, 128, k).transpose(0, 1).reshape(2 * blocks * 128, k).contiguous())
+
+
+@pytest.mark.parametrize("act,limit", [("silu", 0.0), ("relu", 0.0), ("clamped", 1.5), ("gelu_tanh", 0.0)])
+@pytest.mark.parametrize("m,i,k", [(1, 5632, 2048), (3, 1, 130), (16, 128, 512), (17, 1000, 300), (40, 300, 2000), (64, 2050, 256), (70, 200, 1111),
+                                   (128, 640, 384), (129, 129, 500), (300, 1000, 640), (1300, 777, 260)])
+def test_gated_products(ops, m, i, k, act, limit):
+    g = rng(m + i + k)
+    a, w = rows8(ops, 2 * randn(g, m, k)), gated_weight(ops, g, i, k)
+    want, off = fu.gated(*a, *w, i, act, limit)
+    wide = torch.full((m, i + 3), 7.0, dtype=torch.bfloat16, device=DEV)
+    for out in (torch.empty(m, i, dtype=torch.bfloat16, device=DEV), wide[:, :i]):
+        ops.linear_swiglu_fp8(*a, *w, out, act=act, limit=limit)
+        assert bool(((out.double() - want).abs() <= off + 2.0 ** -8 * (want.abs() + off)).all())
+    assert bool((wide[:, i:] == 7.0).all())
+    room = torch.full((m, -(-i // 16) * 16 + 16), 7, dtype=torch.uint8, device=DEV)
+    scales = torch.full((m, fu.groups(i) + 3), 7, dtype=torch.uint8, device=DEV)
+    out, sc = room.view(ops.FP8)[:, :i], scales.view(ops.FP8_SCALE)[:, : fu.groups(i)]
+    ops.linear_swiglu_fp8(*a, *w, out, sc, act=act, limit=limit)
+    assert fu.between_roundings(out, sc, want, off)
+    assert bool((room[:, i:] == 7).all()) and bool((scales[:, fu.groups(i):] == 7).all())
+    ops.check_status()
+
+
+# ---------------------------------------------------------------------------------------------- together
+
+
+@pytest.mark.parametrize("m", [1, 9, 100, 513])
+def test_a_feed_forward_in_8_bits(ops, m):
+    """Norm, gate and up, down into the stream, one kernel each, on another stream than the default one and captured: the graph
+    does with new rows what the calls do.  Against the same chain in 64 bits from the kernel's own 8-bit rows."""
+    g = rng(m)
+    h, i = 520, 1000
+    x, norm = randn(g, m, h), 1 + 0.2 * randn(g, h)
+    gate_up, down = gated_weight(ops, g, i, h), weight8(ops, randn(g, h, i) / math.sqrt(i))
+    y, mid, out = ops.fp8_rows(m, h, DEV), ops.fp8_rows(m, i, DEV), x.clone()
+
+    def chain():
+        ops.rms_norm_fp8(x, norm, 1e-5, *y)
+        ops.linear_swiglu_fp8(*y, *gate_up, *mid)
+        ops.linear_fp8(*mid, *down, out, accumulate=True)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        chain()
+    torch.cuda.current_stream().wait_stream(side)
+    want, off = fu.product(*mid, *down)
+    assert bool(((out - (x + want)).abs() <= off + 2.0 ** -23 * ((x + want).abs() + want.abs() + off)).all())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        chain()
+    fresh = randn(g, m, h)
+    for rows in (x.clone(), fresh):
+        x.copy_(rows)
+        out.copy_(rows)
+        graph.replay()
+        replayed = out.clone()
+        out.copy_(rows)
+        chain()
+        assert torch.equal(out, replayed)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("m", [1, 50, 300])
+def test_a_weight_may_be_made_right_before_it_is_read(ops, m):
+    """Products begin to read their weight while earlier launches run; the kernel that makes an 8-bit weight does not let them."""
+    g = rng(m)
+    n, k = 4096, 4096
+    a, w = rows8(ops, randn(g, m, k)), [randn(g, n, k) for _ in range(4)]
+    room, out = ops.fp8_weight(n, k, DEV), [torch.empty(m, n, device=DEV) for _ in w]
+    for x, o in zip(w, out):
+        ops.quantize_weight_fp8(x, *room)
+        ops.linear_fp8(*a, *room, o)
+    for x, o in zip(w, out):
+        want, off = fu.product(*a, *weight8(ops, x))
+        assert bool(((o - want).abs() <= off + 2.0 ** -24 * want.abs()).all())
+
+
+def test_no_rows(ops):
+    g = rng(0)
+    w = weight8(ops, randn(g, 256, 128))
+    a = ops.fp8_rows(0, 128, DEV)
+    before = ops.launches
+    ops.quantize_fp8(torch.empty(0, 128, device=DEV), *a)
+    ops.linear_fp8(*a, *w, torch.empty(0, 256, device=DEV))
+    ops.linear_swiglu_fp8(*a, *w, torch.empty(0, 128, dtype=torch.bfloat16, device=DEV))
+    assert ops.launches == before

@@ -1,0 +1,122 @@
+"""What the 8-bit operators refuse, checked without a GPU: the checks run before any kernel is built or launched."""
+import pytest
+import torch
+
+from tiny_llm_b200 import ops
+from tiny_llm_b200.ops import KernelError
+
+
+@pytest.fixture
+def no_device(monkeypatch):
+    """The checks of shapes and types on CPU tensors; a call that passes them all ends at the (missing) launch."""
+    monkeypatch.setattr(ops, "_fp8_here", lambda *a: None)
+
+    def reached(*_a, **_k):
+        raise LookupError("launched")
+    monkeypatch.setattr(ops.build, "load_library", reached)
+
+
+def rows(m, k):
+    return ops.fp8_rows(m, k, "cpu")
+
+
+def weight(n, k):
+    return ops.fp8_weight(n, k, "cpu")
+
+
+def test_room_for_rows_and_weights():
+    data, scales = rows(3, 130)
+    assert data.shape == (3, 130) and data.stride() == (144, 1) and data.dtype == torch.float8_e4m3fn
+    assert scales.shape == (3, 2) and scales.dtype == torch.float8_e8m0fnu
+    data, scales = weight(257, 128)
+    assert data.shape == (257, 128) and data.is_contiguous() and scales.shape == (3, 1) and scales.dtype == torch.float32
+
+
+def test_tensors_on_the_host_are_refused():
+    a, w = rows(2, 128), weight(128, 128)
+    for call in (lambda: ops.quantize_fp8(torch.zeros(2, 128), *a), lambda: ops.quantize_weight_fp8(torch.zeros(128, 128), *w),
+                 lambda: ops.rms_norm_fp8(torch.zeros(2, 128), torch.zeros(128), 1e-5, *a),
+                 lambda: ops.linear_fp8(*a, *w, torch.zeros(2, 128)),
+                 lambda: ops.linear_swiglu_fp8(*a, *weight(256, 128), torch.zeros(2, 128, dtype=torch.bfloat16))):
+        with pytest.raises(KernelError, match="CUDA device only"):
+            call()
+
+
+def test_calls_that_fit_reach_their_kernel(no_device):
+    a, w = rows(2, 200), weight(300, 200)
+    wide = torch.zeros(2, 320)
+    for call in (lambda: ops.quantize_fp8(torch.zeros(2, 300)[:, 100:], *a), lambda: ops.quantize_fp8(torch.zeros(2, 200, dtype=torch.bfloat16), *a),
+                 lambda: ops.quantize_weight_fp8(torch.zeros(300, 200), *w),
+                 lambda: ops.rms_norm_fp8(torch.zeros(9, 200), torch.zeros(200), 1e-5, *a, rows=torch.zeros(2, dtype=torch.int32)),
+                 lambda: ops.linear_fp8(*a, *w, wide[:, :300]), lambda: ops.linear_fp8(*a, *w, wide[:, 20:], accumulate=True),
+                 lambda: ops.linear_fp8(a[0][:1], a[1][:1], *w, torch.zeros(1, 300, dtype=torch.bfloat16)),
+                 lambda: ops.linear_swiglu_fp8(*a, *weight(512, 200), *rows(2, 130)),
+                 lambda: ops.linear_swiglu_fp8(*a, *weight(512, 200), torch.zeros(2, 256, dtype=torch.bfloat16), act="clamped", limit=1.0)):
+        with pytest.raises(Exception) as e:
+            call()
+        assert isinstance(e.value, LookupError) or "CUDA" in str(e.value) or "NVIDIA" in str(e.value), e.value
+
+
+def test_rows_and_weights_that_do_not_fit(no_device):
+    a, w = rows(2, 200), weight(300, 200)
+    bad_start = torch.zeros(2 * 208 + 8, dtype=torch.uint8)[8:].view(torch.float8_e4m3fn).view(2, 208)[:, :200]
+    if bad_start.data_ptr() % 16 == 0:
+        bad_start = torch.zeros(2 * 208 + 9, dtype=torch.uint8)[9:].view(torch.float8_e4m3fn).view(2, 208)[:, :200]
+    x = torch.zeros(2, 200)
+    bad = [
+        lambda: ops.quantize_fp8(x.half(), *a),                                                   # a type that no kernel takes
+        lambda: ops.quantize_fp8(torch.zeros(200, 2).T, *a),                                      # columns side by side
+        lambda: ops.quantize_fp8(torch.zeros(2, 201), *a),
+        lambda: ops.quantize_fp8(x, torch.empty(2, 200, dtype=torch.float8_e4m3fn), a[1]),        # rows off 16 bytes
+        lambda: ops.quantize_fp8(x, bad_start, a[1]),
+        lambda: ops.quantize_fp8(x, a[0].view(torch.uint8), a[1]),
+        lambda: ops.quantize_fp8(x, a[0].view(torch.uint8).view(torch.float8_e5m2), a[1]),
+        lambda: ops.quantize_fp8(x, a[0], torch.zeros(2, 2)),                                     # scales of another type, shape, order
+        lambda: ops.quantize_fp8(x, a[0], rows(2, 300)[1]),
+        lambda: ops.quantize_fp8(x, a[0], torch.empty(2, 2, dtype=torch.float8_e8m0fnu).T),
+        lambda: ops.quantize_fp8(x, a[0][:1].expand(2, 200), a[1]),                               # one row twice
+        lambda: ops.quantize_fp8(x, a[0], a[1][:1].expand(2, 2)),
+        lambda: ops.quantize_weight_fp8(torch.zeros(300, 200), w[0], w[1].double()),
+        lambda: ops.quantize_weight_fp8(torch.zeros(300, 200), w[0], torch.zeros(3, 3)[:, :2]),
+        lambda: ops.quantize_weight_fp8(torch.zeros(200, 300).T, *w),
+        lambda: ops.rms_norm_fp8(x.bfloat16(), torch.zeros(200), 1e-5, *a),
+        lambda: ops.rms_norm_fp8(torch.zeros(2, 300)[:, :200], torch.zeros(200), 1e-5, *a),
+        lambda: ops.rms_norm_fp8(x, torch.zeros(199), 1e-5, *a),
+        lambda: ops.rms_norm_fp8(torch.zeros(5, 200), torch.zeros(200), 1e-5, *a),
+        lambda: ops.rms_norm_fp8(x, torch.zeros(200), 1e-5, *a, rows=torch.zeros(2, dtype=torch.int64)),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(KernelError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+
+
+def test_products_that_do_not_fit(no_device):
+    a, w, out = rows(2, 200), weight(300, 200), torch.zeros(2, 300)
+    half = torch.bfloat16
+    bad = [
+        lambda: ops.linear_fp8(*rows(2, 208), *w, out),
+        lambda: ops.linear_fp8(*a, *w, out[:, :299]),
+        lambda: ops.linear_fp8(*a, *w, torch.zeros(3, 300)),
+        lambda: ops.linear_fp8(*a, *w, out.half()),
+        lambda: ops.linear_fp8(*a, *w, out.to(half), accumulate=True),
+        lambda: ops.linear_fp8(*a, *w, torch.zeros(300, 2).T),
+        lambda: ops.linear_fp8(*a, *w, out[:1].expand(2, 300)),
+        lambda: ops.linear_fp8(a[0], w[1], *w, out),
+        lambda: ops.linear_fp8(*a, w[0], w[1][:2], out),
+        lambda: ops.linear_fp8(*a, w[0], w[1].T.contiguous().T, out),
+        lambda: ops.linear_fp8(a[0].expand(2, 200)[:1].expand(2, 200), a[1], *w, out),
+        lambda: ops.linear_fp8(*rows(2, 0), *weight(300, 0), out),
+        lambda: ops.linear_swiglu_fp8(*a, *weight(512, 200), torch.zeros(2, 128, dtype=half)),    # rows for another width
+        lambda: ops.linear_swiglu_fp8(*a, *weight(400, 200), torch.zeros(2, 200, dtype=half)),    # blocks that are not filled
+        lambda: ops.linear_swiglu_fp8(*a, *weight(512, 200), torch.zeros(2, 200)),
+        lambda: ops.linear_swiglu_fp8(*a, *weight(512, 200), rows(2, 200)[0]),
+        lambda: ops.linear_swiglu_fp8(*a, *weight(512, 200), torch.zeros(2, 200, dtype=half), rows(2, 200)[1]),
+        lambda: ops.linear_swiglu_fp8(*a, *weight(512, 200), torch.zeros(2, 200, dtype=half), act="tanh"),
+        lambda: ops.linear_swiglu_fp8(*a, *weight(512, 200), torch.zeros(2, 200, dtype=half), act="clamped"),
+        lambda: ops.linear_swiglu_fp8(*a, *weight(512, 200), torch.zeros(3, 200, dtype=half)),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(KernelError):
+            call()
+            pytest.fail(f"call {i} was not refused")

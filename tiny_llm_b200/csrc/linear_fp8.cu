@@ -1,0 +1,357 @@
+// 8-bit matrix products on the tensor cores:
+//   C[m, n] = sum over groups g of 128 values of K:  sa[m, g] * sw[n / 128, g] * sum_{k in g} A[m, k] W[n, k]
+// A [M, K] and W [N, K] are e4m3, sa one e8m0 scale per row and group, sw one float32 scale per block of 128 x 128.
+//
+// The products of a group are summed by the tensor cores in 32 bits (tcgen05.mma kind::f8f6f4, four instructions of K = 32) into
+// one of two accumulators in tensor memory.  While they fill the other one, eight warps read it back and add it, times the two
+// scales, to 32-bit sums in registers: the scales of two groups differ, so the groups cannot be added up in tensor memory.  The sums
+// are rounded once, when they leave:
+//   * as bfloat16, as float32, or added to float32 rows;
+//   * gated: the columns of a tile are 128 gate columns and the 128 matching up columns, act(gate) * up leaves as bfloat16 or in 8
+//     bits again, with a scale per row and tile (its 128 columns are one group of the product behind it).
+//
+// Sizes: any M, N and K; rows of A and W start on 16 bytes.  TMA fills the tails with zeros, the epilogue masks them.  Every wait
+// is bounded: on expiry the kernel records a code in `status`, stops issuing, frees its tensor memory and returns.
+#include <map>
+#include <mutex>
+#include <tuple>
+
+#include "fp8.cuh"
+#include "tc_common.cuh"
+
+TLLM_DEFINE_LAST_ERROR
+
+namespace tllm {
+
+constexpr int BM = 128;          // rows of A per CTA = MMA M
+constexpr int BK = FP8_GROUP;    // values of K per stage: one group, one 128-byte swizzle row
+constexpr int UMMA_K = 32;
+constexpr int SUM_WARPS = 8;     // warps that scale and add: two per 32 rows, half of the columns each
+constexpr int THREADS = 64 + 32 * SUM_WARPS;   // warp 0: TMA, warp 1: MMA + tensor-memory allocation
+
+enum Output { OUT_BF16 = 0, OUT_F32 = 1, OUT_ADD = 2, OUT_FP8 = 3 };
+enum Act { ACT_SILU = 0, ACT_RELU = 1, ACT_CLAMPED = 2, ACT_GELU_TANH = 3 };
+
+struct Fp8Args {
+  const uint8_t* a_scales;     // [m][lda_s] e8m0
+  const float* w_scales;       // [ceil(n / 128)][groups]
+  void* out;
+  uint8_t* out_scales;         // OUT_FP8: [m][ldo_s] e8m0
+  long long lda_s, ldo, ldo_s;
+  int m, n, groups;            // n: columns of `out` (gated: half the weight's rows, without the ones that fill the last block)
+  int mode, act;
+  float limit;
+  int vec_out;                 // rows of `out` start on 16 bytes
+};
+
+__device__ __forceinline__ float gate_f(float g, float u, int act, float limit) {
+  if (act == ACT_SILU) return g / (1.f + expf(-g)) * u;
+  if (act == ACT_RELU) return fmaxf(g, 0.f) * u;
+  if (act == ACT_CLAMPED) {
+    g = fminf(g, limit);
+    u = fminf(fmaxf(u, -limit), limit);
+    return g / (1.f + expf(-1.702f * g)) * (u + 1.f);
+  }
+  return g / (1.f + expf(-1.59576912160573081f * g * fmaf(0.044715f * g, g, 1.f))) * u;   // 2 sqrt(2 / pi)
+}
+
+// e4m3 x e4m3 -> float32, M = m, N = n, both operands K-major (bits 7-9 and 10-12: 0 is e4m3)
+__device__ __forceinline__ uint32_t instr_desc_e4m3(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+__device__ __forceinline__ void umma_fp8_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(SMEM_DESC_SW128_HI) : "memory");
+}
+// true in all the summing warps only if `ok` holds in all of them
+__device__ __forceinline__ bool sums_all(bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %1, 0;\n\t"
+      "bar.red.and.pred p, 1, %2, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r) : "r"((uint32_t)ok), "n"(32 * SUM_WARPS) : "memory");
+  return r != 0;
+}
+
+template <int BN, int STAGES>
+struct Smem {
+  static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int MOST_OFFSET = STAGES * STAGE_BYTES;           // the largest magnitudes of a row's two halves
+  static constexpr int BAR_OFFSET = MOST_OFFSET + 2 * BM * 4;
+  static constexpr int TOTAL = BAR_OFFSET + (2 * STAGES + 4) * 8 + 16 + 1024;
+};
+
+// eight columns as bfloat16
+__device__ __forceinline__ uint4 pack8_bf16(const float* v) {
+  uint4 pk;
+  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&pk);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+  return pk;
+}
+
+// `N` columns of this thread's row from column `n` on, as `mode` says
+template <int N>
+__device__ __forceinline__ void store_columns(const Fp8Args& p, int m, int n, const float* v, int mode) {
+  if (m >= p.m || n >= p.n) return;
+  const bool full = n + N <= p.n && p.vec_out;
+  if (mode == OUT_BF16) {
+    __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + (size_t)m * p.ldo + n;
+    if (full) {
+#pragma unroll
+      for (int j = 0; j < N; j += 8) *reinterpret_cast<uint4*>(dst + j) = pack8_bf16(v + j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (n + j < p.n) dst[j] = __float2bfloat16_rn(v[j]);
+    }
+  } else {
+    float* dst = reinterpret_cast<float*>(p.out) + (size_t)m * p.ldo + n;
+    if (full) {
+#pragma unroll
+      for (int j = 0; j < N; j += 4) {
+        float4 o = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        if (mode == OUT_ADD) {
+          const float4 r = *reinterpret_cast<const float4*>(dst + j);
+          o.x += r.x; o.y += r.y; o.z += r.z; o.w += r.w;
+        }
+        *reinterpret_cast<float4*>(dst + j) = o;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (n + j < p.n) dst[j] = mode == OUT_ADD ? dst[j] + v[j] : v[j];
+    }
+  }
+}
+
+template <int BN, int STAGES, bool GATED>
+__global__ void __launch_bounds__(THREADS, 1)
+linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const Fp8Args p, int* __restrict__ status) {
+  static_assert(!GATED || BN == 256, "a gated tile is one group of gate columns and one of up columns");
+  using L = Smem<BN, STAGES>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint32_t* most = reinterpret_cast<uint32_t*>(smem + L::MOST_OFFSET);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::BAR_OFFSET);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* acc_full = empty_bar + STAGES;      // [2]: accumulator b holds a group's products
+  uint64_t* acc_empty = acc_full + 2;           // [2]: the summing warps have read accumulator b
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles_m = (p.m + BM - 1) / BM, tiles_n = GATED ? (p.n + 127) / 128 : (p.n + BN - 1) / BN;
+  const int n_tiles = tiles_m * tiles_n;
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_map(&map_a); tma_prefetch_map(&map_w);
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], SUM_WARPS); }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, 2 * BN);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_trigger();
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------- TMA producer
+      int it = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x)
+        for (int g = 0; g < p.groups; ++g, ++it) {
+          const int s = it % STAGES;
+          if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { *abort_flag = 1; atomicExch(status, ERR_F8_PRODUCER); ok = false; break; }
+          uint8_t* dst = smem + s * L::STAGE_BYTES;
+          mbar_expect_tx(&full_bar[s], L::STAGE_BYTES);
+          tma_load_2d(dst, &map_a, g * BK, (t % tiles_m) * BM, &full_bar[s]);
+          tma_load_2d(dst + L::A_BYTES, &map_w, g * BK, (t / tiles_m) * BN, &full_bar[s]);
+        }
+      mbar_drain(full_bar, STAGES, it);
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (warp-wide loop, one elected lane issues)
+    const uint32_t idesc = instr_desc_e4m3(BM, BN);
+    const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
+    const uint32_t lo0 = smem_desc_sw128_lo(smem_u32(smem));
+    int it = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x)
+      for (int g = 0; g < p.groups; ++g, ++it) {
+        const int s = it % STAGES, buf = it & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, abort_flag) && mbar_wait(&full_bar[s], (it / STAGES) & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t a_lo = lo0 + s * (L::STAGE_BYTES >> 4), b_lo = a_lo + (L::A_BYTES >> 4);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k)
+            umma_fp8_lo(tmem_u + buf * BN, a_lo + (k * UMMA_K >> 4), b_lo + (k * UMMA_K >> 4), idesc, k > 0 ? 1u : 0u);
+          umma_commit(&empty_bar[s]);
+          umma_commit(&acc_full[buf]);
+        }
+        __syncwarp();
+      }
+    if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_MMA); }
+  } else {
+    // ---------------- sums: warp w reads tensor-memory lanes [32 (w % 4), +32), and of its row half the columns: with a plain
+    // tile [half * BN / 2, +BN / 2), with a gated one 64 gate columns and the 64 matching up columns
+    constexpr int COLS = BN / 2, CHUNKS = COLS / 32;
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    const int row = quad * 32 + lane;
+    auto column = [&](int c) { return GATED ? (c < CHUNKS / 2 ? half * 64 + 32 * c : 128 + half * 64 + 32 * (c - CHUNKS / 2)) : half * COLS + 32 * c; };
+    int it = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < n_tiles; t += gridDim.x) {
+      const int m = (t % tiles_m) * BM + row, tile_n = t / tiles_m;
+      const uint8_t* sa = p.a_scales + (long long)min(m, p.m - 1) * p.lda_s;
+      // the rows of W that a thread reads lie in one block of 128 (gated: one of gate, one of up), the last one where W ends inside a tile
+      const int block = GATED ? 2 * tile_n : min((tile_n * BN + half * COLS) / 128, (p.n - 1) / 128);
+      const float* sw = p.w_scales + (long long)block * p.groups;
+      float acc[COLS];
+#pragma unroll
+      for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
+      for (int g = 0; g < p.groups; ++g, ++it) {
+        const int buf = it & 1;
+        const float a = fp8_scale(sa[g]), s0 = a * sw[g], s1 = GATED ? a * sw[p.groups + g] : s0;
+        ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (it >> 1) & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t taddr = tmem_base + buf * BN + ((uint32_t)(quad * 32) << 16);
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+          float v[32];
+          tmem_ld32(taddr + column(c), v);
+          const float s = GATED && c >= CHUNKS / 2 ? s1 : s0;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[32 * c + j] = fmaf(v[j], s, acc[32 * c + j]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      }
+      if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_SUMS); }
+      if (!sums_all(ok)) break;
+      if (!GATED) {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) store_columns<32>(p, m, tile_n * BN + column(c), acc + 32 * c, p.mode);
+      } else {
+        const int n = tile_n * 128 + half * 64;
+#pragma unroll
+        for (int j = 0; j < 64; ++j) acc[j] = n + j < p.n ? gate_f(acc[j], acc[64 + j], p.act, p.limit) : 0.f;
+        if (p.mode != OUT_FP8) {
+          store_columns<32>(p, m, n, acc, OUT_BF16);
+          store_columns<32>(p, m, n + 32, acc + 32, OUT_BF16);
+        } else {
+          uint32_t largest = 0u;
+#pragma unroll
+          for (int j = 0; j < 64; ++j) largest = max(largest, fp8_abs_bits(acc[j]));
+          most[half * BM + row] = largest;
+          sums_all(true);
+          const uint32_t byte = fp8_scale_byte(max(most[row], most[BM + row]));
+          const float inverse = fp8_inverse_scale(byte);
+          if (m < p.m) {
+            uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + (size_t)m * p.ldo + n;
+            if (half == 0) p.out_scales[(size_t)m * p.ldo_s + tile_n] = (uint8_t)byte;
+#pragma unroll
+            for (int j = 0; j < 64; j += 16) {
+              uint4 pk;
+              pk.x = fp8_pack4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3], inverse);
+              pk.y = fp8_pack4(acc[j + 4], acc[j + 5], acc[j + 6], acc[j + 7], inverse);
+              pk.z = fp8_pack4(acc[j + 8], acc[j + 9], acc[j + 10], acc[j + 11], inverse);
+              pk.w = fp8_pack4(acc[j + 12], acc[j + 13], acc[j + 14], acc[j + 15], inverse);
+              if (n + j + 16 <= p.n) {
+                *reinterpret_cast<uint4*>(dst + j) = pk;
+              } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  if (n + j + e < p.n) dst[j + e] = (uint8_t)((&pk.x)[e / 4] >> (8 * (e % 4)));
+              }
+            }
+          }
+          sums_all(true);   // the next tile's largest magnitudes wait for this one's readers
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem_base, 2 * BN);
+}
+
+// ---------------------------------------------------------------- host side
+// A 2-D tensor of bytes [rows, k] with row stride ld, tiled in boxes of box_rows x 128.
+static bool make_map(CUtensorMap* map, const void* ptr, int rows, int k, long long ld, int box_rows) {
+  using Key = std::tuple<const void*, int, int, long long, int>;
+  static std::map<Key, CUtensorMap> cache;
+  static std::mutex mu;
+  const Key key(ptr, rows, k, ld, box_rows);
+  std::lock_guard<std::mutex> lock(mu);
+  auto it = cache.find(key);
+  if (it != cache.end()) { *map = it->second; return true; }
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {(cuuint32_t)BK, (cuuint32_t)box_rows};
+  cuuint32_t elem[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return false;
+  if (cache.size() > 4096) cache.clear();
+  cache[key] = *map;
+  return true;
+}
+
+template <int BN, int STAGES, bool GATED>
+static int launch_tiles(const Fp8Args& p, const void* a, long long lda, const void* w, long long ldw, int w_rows, int k, int* status, cudaStream_t s) {
+  using L = Smem<BN, STAGES>;
+  auto kern = linear_fp8_kernel<BN, STAGES, GATED>;
+  TLLM_RESERVE_SMEM("linear_fp8", L::TOTAL, kern);
+  CUtensorMap ma, mw;
+  if (!make_map(&ma, a, p.m, k, lda, BM) || !make_map(&mw, w, w_rows, k, ldw, BN)) TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: cannot describe the operands to the copy unit");
+  const int tiles = ((p.m + BM - 1) / BM) * (GATED ? (p.n + 127) / 128 : (p.n + BN - 1) / BN);
+  int dev = 0, sm_count = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sm_count < 1)
+    TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: cannot read the number of SMs");
+  TLLM_LAUNCH("linear_fp8", kern, tiles < sm_count ? tiles : sm_count, THREADS, L::TOTAL, s, ma, mw, p, status);
+  return TLLM_OK;
+}
+
+}  // namespace tllm
+
+using namespace tllm;
+
+// gated: `n` is the number of output columns, w has 256 * ceil(n / 128) rows; else w has n rows.
+extern "C" int tllm_linear_fp8(const void* a, long long lda, const void* a_scales, long long lda_s, const void* w, long long ldw,
+                               const float* w_scales, void* out, long long ldo, void* out_scales, long long ldo_s, int m, int n, int k,
+                               int mode, int gated, int act, float limit, int* status, void* stream) {
+  TLLM_REQUIRE(m > 0 && n > 0 && k > 0, "linear_fp8: empty product");
+  TLLM_REQUIRE((uintptr_t)a % 16 == 0 && (uintptr_t)w % 16 == 0 && lda % 16 == 0 && ldw % 16 == 0 && lda >= k && ldw >= k,
+               "linear_fp8: rows of 8-bit values start on 16 bytes");
+  TLLM_REQUIRE(gated ? (mode == OUT_BF16 || mode == OUT_FP8) : (mode >= OUT_BF16 && mode <= OUT_ADD), "linear_fp8: output code %d", mode);
+  TLLM_REQUIRE(act >= 0 && act <= 3 && (act != ACT_CLAMPED || limit > 0.f), "linear_fp8: activation code %d, limit %g", act, (double)limit);
+  Fp8Args p = {};
+  p.a_scales = (const uint8_t*)a_scales; p.w_scales = w_scales; p.out = out; p.out_scales = (uint8_t*)out_scales;
+  p.lda_s = lda_s; p.ldo = ldo; p.ldo_s = ldo_s;
+  p.m = m; p.n = n; p.groups = (k + BK - 1) / BK;
+  p.mode = mode; p.act = act; p.limit = limit;
+  const int size = mode == OUT_BF16 ? 2 : (mode == OUT_FP8 ? 1 : 4);
+  p.vec_out = (uintptr_t)out % 16 == 0 && (ldo * size) % 16 == 0;
+  TLLM_REQUIRE(mode != OUT_FP8 || p.vec_out, "linear_fp8: rows of 8-bit values start on 16 bytes");
+  cudaStream_t s = (cudaStream_t)stream;
+  if (gated) return launch_tiles<256, 4, true>(p, a, lda, w, ldw, 256 * ((n + 127) / 128), k, status, s);
+  return launch_tiles<128, 6, false>(p, a, lda, w, ldw, n, k, status, s);
+}

@@ -1233,7 +1233,8 @@ _STATUS_CODES = {1: "TMA producer of a tensor-core product", 2: "MMA issuer of a
                  12: "copying warp of a delta-rule or state-space scan", 13: "computing warp of a delta-rule or state-space scan",
                  14: "TMA producer of a 32-bit tensor-core product", 15: "MMA issuer of a 32-bit tensor-core product",
                  16: "splitting warp of a 32-bit tensor-core product", 17: "summing warp of a 32-bit tensor-core product",
-                 18: "TMA producer of the attention of decoded tokens", 19: "computing warp of the attention of decoded tokens"}
+                 18: "TMA producer of the attention of decoded tokens", 19: "computing warp of the attention of decoded tokens",
+                 20: "TMA producer of an 8-bit product", 21: "MMA issuer of an 8-bit product", 22: "summing warp of an 8-bit product"}
 
 
 def raise_status(device, code: int) -> None:
@@ -1482,6 +1483,187 @@ def linear_swiglu(a: torch.Tensor, w_gate_up: torch.Tensor, out: torch.Tensor, b
     gu = workspace.get("gate_up", (m, n2), a.dtype)
     linear(a, w_gate_up, gu)
     silu_mul(gu, out, block, act=act, limit=limit)
+
+
+# ----------------------------------------------------------------------------- 8-bit products
+
+# e4m3 values with a scale per group of 128: activations [M, K] carry one e8m0 scale (a power of two) per row and group of
+# K, weights [N, K] one float32 scale per block of 128 x 128.  A scale that the ops below make is the smallest power of two
+# that brings the largest magnitude of its group to 448 or less, 2^-126 at least, and 1 for a group of zeros; a group that
+# holds an infinity or a NaN has the scale NaN and the values 0, so that whatever is computed from it is NaN.
+FP8_GROUP = 128
+FP8, FP8_SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
+OUT_FP8 = 3
+
+
+def _fp8_groups(k: int) -> int:
+    return -(-k // FP8_GROUP)
+
+
+def fp8_rows(m: int, k: int, device):
+    """Room for 8-bit rows: (values e4m3 [m, k], whose rows start on 16 bytes, and scales e8m0 [m, ceil(k / 128)]).  The
+    values are a view where k is no multiple of 16; what lies behind a row's end is never read or written."""
+    data = torch.empty(m, -(-k // 16) * 16, dtype=FP8, device=device)[:, :k]
+    return data, torch.empty(m, _fp8_groups(k), dtype=FP8_SCALE, device=device)
+
+
+def fp8_weight(n: int, k: int, device):
+    """Room for an 8-bit weight: (values e4m3 [n, k], whose rows start on 16 bytes, and scales float32
+    [ceil(n / 128), ceil(k / 128)])."""
+    data = torch.empty(n, -(-k // 16) * 16, dtype=FP8, device=device)[:, :k]
+    return data, torch.empty(_fp8_groups(n), _fp8_groups(k), dtype=torch.float32, device=device)
+
+
+def _fp8_here(name: str, *tensors) -> None:
+    """All on the device whose stream the launch goes to."""
+    _need_cuda(*tensors)
+    here = torch._C._cuda_getDevice()
+    if any(t is not None and t.get_device() != here for t in tensors):
+        raise KernelError(f"{name}: every tensor has to be on the current device, cuda:{here}")
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """The distance of rows in values; of a single row, whose stride means nothing, what a packed one would have."""
+    return t.stride(0) if t.shape[0] > 1 else -(-max(t.shape[1], 1) // 16) * 16
+
+
+def _fp8_values(name: str, t: torch.Tensor, what: str) -> None:
+    if t.dim() != 2 or t.dtype != FP8 or (t.shape[1] > 1 and t.stride(1) != 1) or t.data_ptr() % 16 or _row_stride(t) % 16 or \
+            _row_stride(t) < t.shape[1]:
+        raise KernelError(f"{name}: {what} must be a float8_e4m3fn matrix whose rows start on 16 bytes, got {tuple(t.shape)} "
+                          f"{t.dtype} with strides {t.stride()}")
+
+
+def _fp8_row_scales(name: str, t: torch.Tensor, values: torch.Tensor) -> None:
+    want = (values.shape[0], _fp8_groups(values.shape[1]))
+    if t.dtype != FP8_SCALE or tuple(t.shape) != want or (want[1] > 1 and t.stride(1) != 1) or _row_stride(t) < want[1]:
+        raise KernelError(f"{name}: scales of rows must be a float8_e8m0fnu matrix {want}, got {tuple(t.shape)} {t.dtype} with "
+                          f"strides {t.stride()}")
+
+
+def _fp8_weight_scales(name: str, t: torch.Tensor, values: torch.Tensor) -> None:
+    want = (_fp8_groups(values.shape[0]), _fp8_groups(values.shape[1]))
+    if t.dtype != torch.float32 or tuple(t.shape) != want or not t.is_contiguous():
+        raise KernelError(f"{name}: scales of a weight must be a contiguous float32 matrix {want}, got {tuple(t.shape)} {t.dtype}")
+
+
+def quantize_fp8(x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor) -> None:
+    """Rows of bfloat16 or float32 (a slice of wider rows is fine) to 8-bit rows: out e4m3 [M, K], scales e8m0
+    [M, ceil(K / 128)], as `fp8_rows` makes them."""
+    _fp8_here("quantize_fp8", x, out, scales)
+    if x.dim() != 2 or x.shape != out.shape or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise KernelError(f"quantize_fp8: shapes do not fit: x {tuple(x.shape)} with strides {x.stride()}, out {tuple(out.shape)}")
+    _fp8_values("quantize_fp8", out, "out")
+    _fp8_row_scales("quantize_fp8", scales, out)
+    code = _code(x.dtype)
+    m, k = x.shape
+    if not m or not k:
+        return
+    lib = build.load_library("fp8_quantize")
+    _call(lib, lib.tllm_quantize_fp8, _ptr(x), ctypes.c_longlong(x.stride(0)), _ptr(out), ctypes.c_longlong(_row_stride(out)),
+          _ptr(scales), ctypes.c_longlong(_row_stride(scales)), m, k, code, _stream())
+
+
+def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: torch.Tensor, scales: torch.Tensor,
+                 rows: Optional[torch.Tensor] = None) -> None:
+    """`rms_norm` (x and weight float32, statistics in 32 bits) whose rows leave in 8 bits, rounded from 32: out e4m3
+    [M, K], scales e8m0 [M, ceil(K / 128)].  `rows` (int32): which rows of x are taken."""
+    _fp8_here("rms_norm_fp8", x, weight, out, scales, rows)
+    _i32(rows, "rows")
+    if x.dim() != 2 or out.dim() != 2 or x.dtype != torch.float32 or weight.dtype != torch.float32 or not x.is_contiguous() or \
+            not weight.is_contiguous() or out.shape[1] != x.shape[1] or weight.numel() != x.shape[1] or \
+            out.shape[0] != (x.shape[0] if rows is None else rows.numel()):
+        raise KernelError("rms_norm_fp8: shapes or dtypes do not fit")
+    _fp8_values("rms_norm_fp8", out, "out")
+    _fp8_row_scales("rms_norm_fp8", scales, out)
+    m, k = out.shape
+    if not m or not k:
+        return
+    lib = build.load_library("fp8_quantize")
+    _call(lib, lib.tllm_rms_norm_fp8, _ptr(x), _ptr(weight), _ptr(out), ctypes.c_longlong(_row_stride(out)), _ptr(scales),
+          ctypes.c_longlong(_row_stride(scales)), _ptr(rows), m, k, ctypes.c_float(eps), _stream())
+
+
+def quantize_weight_fp8(w: torch.Tensor, out: torch.Tensor, scales: torch.Tensor) -> None:
+    """A weight [N, K] of bfloat16 or float32 to 8 bits: out e4m3 [N, K], scales float32 [ceil(N / 128), ceil(K / 128)], one
+    per block of 128 x 128, as `fp8_weight` makes them."""
+    _fp8_here("quantize_weight_fp8", w, out, scales)
+    if w.dim() != 2 or w.shape != out.shape or (w.shape[1] > 1 and w.stride(1) != 1):
+        raise KernelError(f"quantize_weight_fp8: shapes do not fit: w {tuple(w.shape)} with strides {w.stride()}, out {tuple(out.shape)}")
+    _fp8_values("quantize_weight_fp8", out, "out")
+    _fp8_weight_scales("quantize_weight_fp8", scales, out)
+    code = _code(w.dtype)
+    n, k = w.shape
+    if not n or not k:
+        return
+    lib = build.load_library("fp8_quantize")
+    _call(lib, lib.tllm_quantize_weight_fp8, _ptr(w), ctypes.c_longlong(w.stride(0)), _ptr(out), ctypes.c_longlong(_row_stride(out)),
+          _ptr(scales), n, k, code, _stream())
+
+
+def _fp8_product(name: str, a, a_scales, w, w_scales) -> None:
+    _fp8_values(name, a, "a")
+    _fp8_values(name, w, "the weight")
+    if w.shape[1] != a.shape[1]:
+        raise KernelError(f"{name}: shapes do not fit: a {tuple(a.shape)}, w {tuple(w.shape)}")
+    if not a.shape[1]:
+        raise KernelError(f"{name}: rows of no values")
+    _fp8_row_scales(name, a_scales, a)
+    _fp8_weight_scales(name, w_scales, w)
+
+
+def _fp8_call(a, a_scales, w, w_scales, out, out_scales, mode, gated=False, act=0, limit=0.0) -> None:
+    lib = build.load_library("linear_fp8")
+    m, n = out.shape
+    _call(lib, lib.tllm_linear_fp8, _ptr(a), ctypes.c_longlong(_row_stride(a)), _ptr(a_scales), ctypes.c_longlong(_row_stride(a_scales)),
+          _ptr(w), ctypes.c_longlong(_row_stride(w)), _ptr(w_scales), _ptr(out),
+          ctypes.c_longlong(out.stride(0) if mode != OUT_FP8 and m > 1 else _row_stride(out)), _ptr(out_scales),
+          ctypes.c_longlong(0 if out_scales is None else _row_stride(out_scales)), m, n, a.shape[1], mode, int(gated), act,
+          ctypes.c_float(limit), _ptr(status_word(a.device)), _stream())
+
+
+def linear_fp8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
+               accumulate: bool = False) -> None:
+    """out = a . w^T of 8-bit operands (a e4m3 [M, K] with e8m0 scales [M, ceil(K / 128)], w e4m3 [N, K] with float32 scales
+    [ceil(N / 128), ceil(K / 128)] of any value), summed in 32 bits on the tensor cores and rounded once to `out` (bfloat16 or
+    float32); accumulate=True adds the product into a float32 `out`.  Any M, N and K; rows of a and w start on 16 bytes.
+    `w` and its scales are taken for a loaded weight (see `linear`): `quantize_weight_fp8` may come right before, but no
+    other launch of this package that still runs may be writing them."""
+    _fp8_here("linear_fp8", a, a_scales, w, w_scales, out)
+    _fp8_product("linear_fp8", a, a_scales, w, w_scales)
+    m, n = a.shape[0], w.shape[0]
+    if tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n) or \
+            out.dtype not in (torch.bfloat16, torch.float32):
+        raise KernelError(f"linear_fp8: out must be bfloat16 or float32 {(m, n)}, got {tuple(out.shape)} {out.dtype} with strides {out.stride()}")
+    if accumulate and out.dtype != torch.float32:
+        raise KernelError("linear_fp8: accumulation needs a float32 output")
+    if not m or not n:
+        return
+    _fp8_call(a, a_scales, w, w_scales, out, None, OUT_ACC if accumulate else (OUT_F32 if out.dtype == torch.float32 else OUT_SAME))
+
+
+def linear_swiglu_fp8(a: torch.Tensor, a_scales: torch.Tensor, w_gate_up: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
+                      out_scales: Optional[torch.Tensor] = None, act: str = "silu", limit: float = 0.0) -> None:
+    """out = act(a Wg^T) * (a Wu^T) of 8-bit operands (as `linear_fp8`), both projections, the activation and the product in one
+    kernel; act one of GLU_ACTS (`limit` belongs to "clamped").  Wg and Wu [I, K] alternate in `w_gate_up` in blocks of 128 rows,
+    zero rows filling the last block of each: 256 * ceil(I / 128) rows.  `out` [M, I] is bfloat16, or e4m3 with e8m0 `out_scales`
+    [M, ceil(I / 128)], rounded from 32 bits: what `linear_fp8` reads next."""
+    _fp8_here("linear_swiglu_fp8", a, a_scales, w_gate_up, w_scales, out, out_scales)
+    _fp8_product("linear_swiglu_fp8", a, a_scales, w_gate_up, w_scales)
+    if act not in GLU_ACTS or (act == "clamped" and not limit > 0):
+        raise KernelError(f"linear_swiglu_fp8: unknown activation {act!r} (known: {', '.join(GLU_ACTS)}; \"clamped\" needs a limit)")
+    if out.dim() != 2 or out.shape[0] != a.shape[0] or w_gate_up.shape[0] != 2 * FP8_GROUP * _fp8_groups(out.shape[1]):
+        raise KernelError(f"linear_swiglu_fp8: shapes do not fit: a {tuple(a.shape)}, w_gate_up {tuple(w_gate_up.shape)}, out {tuple(out.shape)}")
+    m, n = out.shape
+    if out_scales is not None:
+        _fp8_values("linear_swiglu_fp8", out, "out")
+        _fp8_row_scales("linear_swiglu_fp8", out_scales, out)
+    elif out.dtype != torch.bfloat16 or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
+        raise KernelError(f"linear_swiglu_fp8: out must be bfloat16, or e4m3 with out_scales, got {out.dtype} with strides {out.stride()}")
+    if not m or not n:
+        return
+    _fp8_call(a, a_scales, w_gate_up, w_scales, out, out_scales, OUT_FP8 if out_scales is not None else OUT_SAME, True, GLU_ACTS[act],
+              float(limit) if act == "clamped" else 0.0)
 
 
 # ----------------------------------------------------------------------------- attention
@@ -1816,7 +1998,7 @@ def sample(logits: torch.Tensor, work: torch.Tensor, temperature: torch.Tensor, 
                                 _ptr(seeds), _ptr(counters), _ptr(out), _ptr(status), _stream())
 
 
-ALL_LIBRARIES = ("elementwise", "linear_generic", "linear_f32_tc", "linear_tc", "attention_generic", "attention_prep", "recurrence",
+ALL_LIBRARIES = ("elementwise", "linear_generic", "linear_f32_tc", "linear_tc", "linear_fp8", "fp8_quantize", "attention_generic", "attention_prep", "recurrence",
                  "linear_attention", "delta_rule", "head_linear", "window_attention", "attention_talk", "moe", "post_norm", "sampling")
 
 
