@@ -146,8 +146,10 @@ static int check_rows(const char* name, int rows, int width, const void* out, lo
 
 using namespace tllm;
 
-extern "C" int tllm_quantize_fp8(const void* x, long long ldx, void* out, long long ldo, void* scales, long long lds, int rows, int width,
-                                 int dtype, void* stream) {
+// Entry points take their arguments as one struct, which the caller packs in the order of the declaration.
+struct QuantizeCall { const void* x; long long ldx; void* out; long long ldo; void* scales; long long lds; int rows, width, dtype; void* stream; };
+extern "C" int tllm_quantize_fp8(const QuantizeCall* c) {
+  const auto [x, ldx, out, ldo, scales, lds, rows, width, dtype, stream] = *c;
   if (int e = check_rows("quantize_fp8", rows, width, out, ldo, lds)) return e;
   const int groups = (width + FP8_GROUP - 1) / FP8_GROUP;
   const long long blocks = ((long long)rows * groups + ROWS_THREADS / 32 - 1) / (ROWS_THREADS / 32);
@@ -162,8 +164,9 @@ extern "C" int tllm_quantize_fp8(const void* x, long long ldx, void* out, long l
   return TLLM_OK;
 }
 
-extern "C" int tllm_rms_norm_fp8(const float* x, const float* w, void* out, long long ldo, void* scales, long long lds, const int* rows_idx,
-                                 int rows, int width, float eps, void* stream) {
+struct RmsNormCall { const float *x, *w; void* out; long long ldo; void* scales; long long lds; const int* rows_idx; int rows, width; float eps; void* stream; };
+extern "C" int tllm_rms_norm_fp8(const RmsNormCall* c) {
+  const auto [x, w, out, ldo, scales, lds, rows_idx, rows, width, eps, stream] = *c;
   if (int e = check_rows("rms_norm_fp8", rows, width, out, ldo, lds)) return e;
   const int groups = (width + FP8_GROUP - 1) / FP8_GROUP;
   const int vec = (uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0 && width % 4 == 0;
@@ -172,8 +175,9 @@ extern "C" int tllm_rms_norm_fp8(const float* x, const float* w, void* out, long
   return TLLM_OK;
 }
 
-extern "C" int tllm_quantize_weight_fp8(const void* w, long long ldw, void* out, long long ldo, float* scales, int rows, int width, int dtype,
-                                        void* stream) {
+struct QuantizeWeightCall { const void* w; long long ldw; void* out; long long ldo; float* scales; int rows, width, dtype; void* stream; };
+extern "C" int tllm_quantize_weight_fp8(const QuantizeWeightCall* c) {
+  const auto [w, ldw, out, ldo, scales, rows, width, dtype, stream] = *c;
   const int groups = (width + FP8_GROUP - 1) / FP8_GROUP;
   if (int e = check_rows("quantize_weight_fp8", rows, width, out, ldo, groups)) return e;
   const int row_blocks = (rows + FP8_GROUP - 1) / FP8_GROUP;

@@ -335,9 +335,12 @@ static int launch_tiles(const Fp8Args& p, const void* a, long long lda, const vo
 using namespace tllm;
 
 // gated: `n` is the number of output columns, w has 256 * ceil(n / 128) rows; else w has n rows.
-extern "C" int tllm_linear_fp8(const void* a, long long lda, const void* a_scales, long long lda_s, const void* w, long long ldw,
-                               const float* w_scales, void* out, long long ldo, void* out_scales, long long ldo_s, int m, int n, int k,
-                               int mode, int gated, int act, float limit, int* status, void* stream) {
+struct LinearFp8Call {
+  const void* a; long long lda; const void* a_scales; long long lda_s; const void* w; long long ldw; const float* w_scales; void* out; long long ldo;
+  void* out_scales; long long ldo_s; int m, n, k, mode, gated, act; float limit; int* status; void* stream;
+};
+extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
+  const auto [a, lda, a_scales, lda_s, w, ldw, w_scales, out, ldo, out_scales, ldo_s, m, n, k, mode, gated, act, limit, status, stream] = *c;
   TLLM_REQUIRE(m > 0 && n > 0 && k > 0, "linear_fp8: empty product");
   TLLM_REQUIRE((uintptr_t)a % 16 == 0 && (uintptr_t)w % 16 == 0 && lda % 16 == 0 && ldw % 16 == 0 && lda >= k && ldw >= k,
                "linear_fp8: rows of 8-bit values start on 16 bytes");

@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from typing import Optional
 
 import torch
@@ -1514,112 +1515,150 @@ def fp8_weight(n: int, k: int, device):
     return data, torch.empty(_fp8_groups(n), _fp8_groups(k), dtype=torch.float32, device=device)
 
 
-def _fp8_here(name: str, *tensors) -> None:
-    """All on the device whose stream the launch goes to."""
-    _need_cuda(*tensors)
-    here = torch._C._cuda_getDevice()
-    if any(t is not None and t.get_device() != here for t in tensors):
-        raise KernelError(f"{name}: every tensor has to be on the current device, cuda:{here}")
+# The arguments of an entry point travel as one packed struct, in the order and with the types of its C declaration (P: pointer,
+# q: 64 bits, i: 32 bits, f: float): a call of a dozen ctypes objects takes longer than the small kernels.
+_FP8_ENTRIES = {name: (library, struct.Struct(layout)) for name, library, layout in (
+    ("tllm_quantize_fp8", "fp8_quantize", "PqPqPqiiiP"),
+    ("tllm_rms_norm_fp8", "fp8_quantize", "PPPqPqPiifP"),
+    ("tllm_quantize_weight_fp8", "fp8_quantize", "PqPqPiiiP"),
+    ("tllm_linear_fp8", "linear_fp8", "PqPqPqPPqPqiiiiiifPP"))}
+_fp8_loaded = {}
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    """The distance of rows in values; of a single row, whose stride means nothing, what a packed one would have."""
-    return t.stride(0) if t.shape[0] > 1 else -(-max(t.shape[1], 1) // 16) * 16
+def _fp8_call(name: str, *args) -> None:
+    got = _fp8_loaded.get(name)
+    if got is None:
+        library, layout = _FP8_ENTRIES[name]
+        lib = build.load_library(library)
+        got = _fp8_loaded[name] = (lib, getattr(lib, name), layout.pack)
+    _call(got[0], got[1], got[2](*args))
 
 
-def _fp8_values(name: str, t: torch.Tensor, what: str) -> None:
-    if t.dim() != 2 or t.dtype != FP8 or (t.shape[1] > 1 and t.stride(1) != 1) or t.data_ptr() % 16 or _row_stride(t) % 16 or \
-            _row_stride(t) < t.shape[1]:
-        raise KernelError(f"{name}: {what} must be a float8_e4m3fn matrix whose rows start on 16 bytes, got {tuple(t.shape)} "
-                          f"{t.dtype} with strides {t.stride()}")
+def _fp8_here(name: str, *tensors) -> int:
+    """The device that all of them are on, which has to be the current one: its stream gets the launch."""
+    here = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != here or here < 0:
+            _need_cuda(*tensors)
+            raise KernelError(f"{name}: the tensors are on different devices")
+    if here != torch._C._cuda_getDevice():
+        raise KernelError(f"{name}: the tensors are on cuda:{here}, which is not the current device")
+    return here
 
 
-def _fp8_row_scales(name: str, t: torch.Tensor, values: torch.Tensor) -> None:
-    want = (values.shape[0], _fp8_groups(values.shape[1]))
-    if t.dtype != FP8_SCALE or tuple(t.shape) != want or (want[1] > 1 and t.stride(1) != 1) or _row_stride(t) < want[1]:
-        raise KernelError(f"{name}: scales of rows must be a float8_e8m0fnu matrix {want}, got {tuple(t.shape)} {t.dtype} with "
-                          f"strides {t.stride()}")
+def _fp8_misfit(name: str, what: str, t: torch.Tensor) -> KernelError:
+    return KernelError(f"{name}: {what}, got {tuple(t.shape)} {t.dtype} with strides {t.stride()}")
 
 
-def _fp8_weight_scales(name: str, t: torch.Tensor, values: torch.Tensor) -> None:
-    want = (_fp8_groups(values.shape[0]), _fp8_groups(values.shape[1]))
-    if t.dtype != torch.float32 or tuple(t.shape) != want or not t.is_contiguous():
-        raise KernelError(f"{name}: scales of a weight must be a contiguous float32 matrix {want}, got {tuple(t.shape)} {t.dtype}")
+def _fp8_values(name: str, t: torch.Tensor, m: int, k: int) -> int:
+    """The row stride of 8-bit values [m, k] (of a single row, whose stride means nothing, what a packed one would have)."""
+    s0, s1 = t.stride()
+    if m < 2:
+        s0 = -(-k // 16) * 16
+    if t.dtype is not FP8 or (s1 != 1 and k > 1) or s0 & 15 or s0 < k or t.data_ptr() & 15:
+        raise _fp8_misfit(name, "8-bit values are a float8_e4m3fn matrix whose rows start on 16 bytes", t)
+    return s0
+
+
+def _fp8_row_scales(name: str, t: torch.Tensor, m: int, k: int) -> int:
+    """The row stride of the scales of 8-bit rows [m, k]."""
+    g = (k + 127) // 128
+    if t.dtype is not FP8_SCALE or t.shape != (m, g):
+        raise _fp8_misfit(name, f"scales of rows are a float8_e8m0fnu matrix {(m, g)}", t)
+    s0, s1 = t.stride()
+    if m < 2:
+        s0 = g
+    if (s1 != 1 and g > 1) or s0 < g:
+        raise _fp8_misfit(name, "scales of a row stand side by side", t)
+    return s0
+
+
+def _fp8_weight_scales(name: str, t: torch.Tensor, n: int, k: int) -> None:
+    if t.dtype is not torch.float32 or t.shape != ((n + 127) // 128, (k + 127) // 128) or not t.is_contiguous():
+        raise _fp8_misfit(name, f"scales of a weight are a contiguous float32 matrix {((n + 127) // 128, (k + 127) // 128)}", t)
 
 
 def quantize_fp8(x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor) -> None:
     """Rows of bfloat16 or float32 (a slice of wider rows is fine) to 8-bit rows: out e4m3 [M, K], scales e8m0
     [M, ceil(K / 128)], as `fp8_rows` makes them."""
-    _fp8_here("quantize_fp8", x, out, scales)
-    if x.dim() != 2 or x.shape != out.shape or (x.shape[1] > 1 and x.stride(1) != 1):
-        raise KernelError(f"quantize_fp8: shapes do not fit: x {tuple(x.shape)} with strides {x.stride()}, out {tuple(out.shape)}")
-    _fp8_values("quantize_fp8", out, "out")
-    _fp8_row_scales("quantize_fp8", scales, out)
+    here = _fp8_here("quantize_fp8", x, out, scales)
+    shape = x.shape
+    if len(shape) != 2 or shape != out.shape or (x.stride(1) != 1 and shape[1] > 1):
+        raise _fp8_misfit("quantize_fp8", f"x is a matrix of out's shape {tuple(out.shape)}, its rows' values side by side", x)
+    m, k = shape
+    ldo = _fp8_values("quantize_fp8", out, m, k)
+    lds = _fp8_row_scales("quantize_fp8", scales, m, k)
     code = _code(x.dtype)
-    m, k = x.shape
     if not m or not k:
         return
-    lib = build.load_library("fp8_quantize")
-    _call(lib, lib.tllm_quantize_fp8, _ptr(x), ctypes.c_longlong(x.stride(0)), _ptr(out), ctypes.c_longlong(_row_stride(out)),
-          _ptr(scales), ctypes.c_longlong(_row_stride(scales)), m, k, code, _stream())
+    _fp8_call("tllm_quantize_fp8", x.data_ptr(), x.stride(0), out.data_ptr(), ldo, scales.data_ptr(), lds, m, k, code,
+          torch._C._cuda_getCurrentRawStream(here))
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: torch.Tensor, scales: torch.Tensor,
                  rows: Optional[torch.Tensor] = None) -> None:
     """`rms_norm` (x and weight float32, statistics in 32 bits) whose rows leave in 8 bits, rounded from 32: out e4m3
     [M, K], scales e8m0 [M, ceil(K / 128)].  `rows` (int32): which rows of x are taken."""
-    _fp8_here("rms_norm_fp8", x, weight, out, scales, rows)
-    _i32(rows, "rows")
-    if x.dim() != 2 or out.dim() != 2 or x.dtype != torch.float32 or weight.dtype != torch.float32 or not x.is_contiguous() or \
+    if rows is None:
+        here, taken = _fp8_here("rms_norm_fp8", x, weight, out, scales), 0
+    else:
+        here = _fp8_here("rms_norm_fp8", x, weight, out, scales, rows)
+        _i32(rows, "rows")
+        taken = rows.data_ptr()
+    if x.dim() != 2 or out.dim() != 2 or x.dtype is not torch.float32 or weight.dtype is not torch.float32 or not x.is_contiguous() or \
             not weight.is_contiguous() or out.shape[1] != x.shape[1] or weight.numel() != x.shape[1] or \
             out.shape[0] != (x.shape[0] if rows is None else rows.numel()):
-        raise KernelError("rms_norm_fp8: shapes or dtypes do not fit")
-    _fp8_values("rms_norm_fp8", out, "out")
-    _fp8_row_scales("rms_norm_fp8", scales, out)
+        raise _fp8_misfit("rms_norm_fp8", "x and weight are contiguous float32 rows of out's width, as many as out or `rows` has", x)
     m, k = out.shape
+    ldo = _fp8_values("rms_norm_fp8", out, m, k)
+    lds = _fp8_row_scales("rms_norm_fp8", scales, m, k)
     if not m or not k:
         return
-    lib = build.load_library("fp8_quantize")
-    _call(lib, lib.tllm_rms_norm_fp8, _ptr(x), _ptr(weight), _ptr(out), ctypes.c_longlong(_row_stride(out)), _ptr(scales),
-          ctypes.c_longlong(_row_stride(scales)), _ptr(rows), m, k, ctypes.c_float(eps), _stream())
+    _fp8_call("tllm_rms_norm_fp8", x.data_ptr(), weight.data_ptr(), out.data_ptr(), ldo, scales.data_ptr(), lds, taken, m, k, eps,
+          torch._C._cuda_getCurrentRawStream(here))
 
 
 def quantize_weight_fp8(w: torch.Tensor, out: torch.Tensor, scales: torch.Tensor) -> None:
     """A weight [N, K] of bfloat16 or float32 to 8 bits: out e4m3 [N, K], scales float32 [ceil(N / 128), ceil(K / 128)], one
     per block of 128 x 128, as `fp8_weight` makes them."""
-    _fp8_here("quantize_weight_fp8", w, out, scales)
-    if w.dim() != 2 or w.shape != out.shape or (w.shape[1] > 1 and w.stride(1) != 1):
-        raise KernelError(f"quantize_weight_fp8: shapes do not fit: w {tuple(w.shape)} with strides {w.stride()}, out {tuple(out.shape)}")
-    _fp8_values("quantize_weight_fp8", out, "out")
-    _fp8_weight_scales("quantize_weight_fp8", scales, out)
+    here = _fp8_here("quantize_weight_fp8", w, out, scales)
+    shape = w.shape
+    if len(shape) != 2 or shape != out.shape or (w.stride(1) != 1 and shape[1] > 1):
+        raise _fp8_misfit("quantize_weight_fp8", f"w is a matrix of out's shape {tuple(out.shape)}, its rows' values side by side", w)
+    n, k = shape
+    ldo = _fp8_values("quantize_weight_fp8", out, n, k)
+    _fp8_weight_scales("quantize_weight_fp8", scales, n, k)
     code = _code(w.dtype)
-    n, k = w.shape
     if not n or not k:
         return
-    lib = build.load_library("fp8_quantize")
-    _call(lib, lib.tllm_quantize_weight_fp8, _ptr(w), ctypes.c_longlong(w.stride(0)), _ptr(out), ctypes.c_longlong(_row_stride(out)),
-          _ptr(scales), n, k, code, _stream())
+    _fp8_call("tllm_quantize_weight_fp8", w.data_ptr(), w.stride(0), out.data_ptr(), ldo, scales.data_ptr(), n, k, code,
+          torch._C._cuda_getCurrentRawStream(here))
 
 
-def _fp8_product(name: str, a, a_scales, w, w_scales) -> None:
-    _fp8_values(name, a, "a")
-    _fp8_values(name, w, "the weight")
-    if w.shape[1] != a.shape[1]:
-        raise KernelError(f"{name}: shapes do not fit: a {tuple(a.shape)}, w {tuple(w.shape)}")
-    if not a.shape[1]:
-        raise KernelError(f"{name}: rows of no values")
-    _fp8_row_scales(name, a_scales, a)
-    _fp8_weight_scales(name, w_scales, w)
-
-
-def _fp8_call(a, a_scales, w, w_scales, out, out_scales, mode, gated=False, act=0, limit=0.0) -> None:
-    lib = build.load_library("linear_fp8")
-    m, n = out.shape
-    _call(lib, lib.tllm_linear_fp8, _ptr(a), ctypes.c_longlong(_row_stride(a)), _ptr(a_scales), ctypes.c_longlong(_row_stride(a_scales)),
-          _ptr(w), ctypes.c_longlong(_row_stride(w)), _ptr(w_scales), _ptr(out),
-          ctypes.c_longlong(out.stride(0) if mode != OUT_FP8 and m > 1 else _row_stride(out)), _ptr(out_scales),
-          ctypes.c_longlong(0 if out_scales is None else _row_stride(out_scales)), m, n, a.shape[1], mode, int(gated), act,
-          ctypes.c_float(limit), _ptr(status_word(a.device)), _stream())
+def _fp8_product(name: str, here: int, a, a_scales, w, w_scales, out, n: int, out_scales, mode: int, gated: int, act: int, limit: float) -> None:
+    """The checks that the two products share, and the launch.  `n`: columns of `out`."""
+    wn, k = w.shape
+    m = a.shape[0]
+    if a.shape[1] != k or not k:
+        raise _fp8_misfit(name, f"a has rows of the weight's width {k}, at least 1", a)
+    lda, ldw = _fp8_values(name, a, m, k), _fp8_values(name, w, wn, k)
+    lds = _fp8_row_scales(name, a_scales, m, k)
+    _fp8_weight_scales(name, w_scales, wn, k)
+    if mode == OUT_FP8:
+        ldo, ldos, scales_ptr = _fp8_values(name, out, m, n), _fp8_row_scales(name, out_scales, m, n), out_scales.data_ptr()
+    else:
+        ldo, s1 = out.stride()
+        ldos, scales_ptr = 0, 0
+        if (n > 1 and s1 != 1) or (m > 1 and ldo < n):
+            raise _fp8_misfit(name, "out's rows do not overlap and their values stand side by side", out)
+        if m < 2:
+            ldo = -(-n // 16) * 16
+    if not m or not n:
+        return
+    status = _status.get(here)
+    _fp8_call("tllm_linear_fp8", a.data_ptr(), lda, a_scales.data_ptr(), lds, w.data_ptr(), ldw, w_scales.data_ptr(), out.data_ptr(),
+          ldo, scales_ptr, ldos, m, n, k, mode, gated, act, limit, (status_word(a.device) if status is None else status).data_ptr(),
+          torch._C._cuda_getCurrentRawStream(here))
 
 
 def linear_fp8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
@@ -1629,17 +1668,17 @@ def linear_fp8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scale
     float32); accumulate=True adds the product into a float32 `out`.  Any M, N and K; rows of a and w start on 16 bytes.
     `w` and its scales are taken for a loaded weight (see `linear`): `quantize_weight_fp8` may come right before, but no
     other launch of this package that still runs may be writing them."""
-    _fp8_here("linear_fp8", a, a_scales, w, w_scales, out)
-    _fp8_product("linear_fp8", a, a_scales, w, w_scales)
-    m, n = a.shape[0], w.shape[0]
-    if tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n) or \
-            out.dtype not in (torch.bfloat16, torch.float32):
-        raise KernelError(f"linear_fp8: out must be bfloat16 or float32 {(m, n)}, got {tuple(out.shape)} {out.dtype} with strides {out.stride()}")
-    if accumulate and out.dtype != torch.float32:
-        raise KernelError("linear_fp8: accumulation needs a float32 output")
-    if not m or not n:
-        return
-    _fp8_call(a, a_scales, w, w_scales, out, None, OUT_ACC if accumulate else (OUT_F32 if out.dtype == torch.float32 else OUT_SAME))
+    here = _fp8_here("linear_fp8", a, a_scales, w, w_scales, out)
+    dtype = out.dtype
+    if a.dim() != 2 or w.dim() != 2 or out.shape != (a.shape[0], w.shape[0]) or (dtype is not torch.float32 and dtype is not torch.bfloat16):
+        raise _fp8_misfit("linear_fp8", "a, w and out are matrices, out bfloat16 or float32 with a row per row of a and a column per row of w", out)
+    if accumulate:
+        if dtype is not torch.float32:
+            raise KernelError("linear_fp8: accumulation needs a float32 output")
+        mode = OUT_ACC
+    else:
+        mode = OUT_F32 if dtype is torch.float32 else OUT_SAME
+    _fp8_product("linear_fp8", here, a, a_scales, w, w_scales, out, w.shape[0], None, mode, 0, 0, 0.0)
 
 
 def linear_swiglu_fp8(a: torch.Tensor, a_scales: torch.Tensor, w_gate_up: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
@@ -1648,22 +1687,20 @@ def linear_swiglu_fp8(a: torch.Tensor, a_scales: torch.Tensor, w_gate_up: torch.
     kernel; act one of GLU_ACTS (`limit` belongs to "clamped").  Wg and Wu [I, K] alternate in `w_gate_up` in blocks of 128 rows,
     zero rows filling the last block of each: 256 * ceil(I / 128) rows.  `out` [M, I] is bfloat16, or e4m3 with e8m0 `out_scales`
     [M, ceil(I / 128)], rounded from 32 bits: what `linear_fp8` reads next."""
-    _fp8_here("linear_swiglu_fp8", a, a_scales, w_gate_up, w_scales, out, out_scales)
-    _fp8_product("linear_swiglu_fp8", a, a_scales, w_gate_up, w_scales)
+    if out_scales is None:
+        here = _fp8_here("linear_swiglu_fp8", a, a_scales, w_gate_up, w_scales, out)
+        mode, fits = OUT_SAME, out.dtype is torch.bfloat16
+    else:
+        here = _fp8_here("linear_swiglu_fp8", a, a_scales, w_gate_up, w_scales, out, out_scales)
+        mode, fits = OUT_FP8, out.dtype is FP8
     if act not in GLU_ACTS or (act == "clamped" and not limit > 0):
         raise KernelError(f"linear_swiglu_fp8: unknown activation {act!r} (known: {', '.join(GLU_ACTS)}; \"clamped\" needs a limit)")
-    if out.dim() != 2 or out.shape[0] != a.shape[0] or w_gate_up.shape[0] != 2 * FP8_GROUP * _fp8_groups(out.shape[1]):
-        raise KernelError(f"linear_swiglu_fp8: shapes do not fit: a {tuple(a.shape)}, w_gate_up {tuple(w_gate_up.shape)}, out {tuple(out.shape)}")
-    m, n = out.shape
-    if out_scales is not None:
-        _fp8_values("linear_swiglu_fp8", out, "out")
-        _fp8_row_scales("linear_swiglu_fp8", out_scales, out)
-    elif out.dtype != torch.bfloat16 or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
-        raise KernelError(f"linear_swiglu_fp8: out must be bfloat16, or e4m3 with out_scales, got {out.dtype} with strides {out.stride()}")
-    if not m or not n:
-        return
-    _fp8_call(a, a_scales, w_gate_up, w_scales, out, out_scales, OUT_FP8 if out_scales is not None else OUT_SAME, True, GLU_ACTS[act],
-              float(limit) if act == "clamped" else 0.0)
+    if not fits or a.dim() != 2 or w_gate_up.dim() != 2 or out.dim() != 2 or out.shape[0] != a.shape[0] or \
+            w_gate_up.shape[0] != 256 * ((out.shape[1] + 127) // 128):
+        raise _fp8_misfit("linear_swiglu_fp8", f"out is a bfloat16 matrix, or float8_e4m3fn with out_scales, a row per row of a, and the weight has 256 "
+                          f"rows per 128 columns of it (a {tuple(a.shape)}, w_gate_up {tuple(w_gate_up.shape)})", out)
+    _fp8_product("linear_swiglu_fp8", here, a, a_scales, w_gate_up, w_scales, out, out.shape[1], out_scales, mode, 1, GLU_ACTS[act],
+                 float(limit) if act == "clamped" else 0.0)
 
 
 # ----------------------------------------------------------------------------- attention
