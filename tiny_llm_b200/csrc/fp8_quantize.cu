@@ -47,52 +47,83 @@ __device__ __forceinline__ uint32_t largest4(const float* v) {
 
 constexpr int ROWS_THREADS = 256;
 
-// A warp per (row, group): four values per lane.
+// A warp per row and run of four groups: four values per lane and group, the four loads in flight together.
+constexpr int ROWS_RUN = 4;
 template <typename T>
 __global__ void __launch_bounds__(ROWS_THREADS)
 quantize_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ out, long long ldo,
-                     uint8_t* __restrict__ scales, long long lds, int rows, int width, int groups, int vec) {
+                     uint8_t* __restrict__ scales, long long lds, int rows, int width, int groups, int runs, int vec) {
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * (ROWS_THREADS / 32) + (threadIdx.x >> 5);
-  const long long row = item / groups;
-  if (row >= rows) return;
-  const int g = (int)(item - row * groups), k = g * FP8_GROUP + 4 * lane;
-  float v[4];
-  load4(x + row * ldx, k, width, vec, v);
-  const uint32_t byte = fp8_scale_byte(__reduce_max_sync(0xffffffffu, largest4(v)));
-  store4(out + row * ldo, k, width, fp8_pack4(v[0], v[1], v[2], v[3], fp8_inverse_scale(byte)));
-  if (lane == 0) scales[row * lds + g] = (uint8_t)byte;
+  const unsigned item = blockIdx.x * (ROWS_THREADS / 32) + (threadIdx.x >> 5);
+  const unsigned row = item / (unsigned)runs;
+  if (row >= (unsigned)rows) return;
+  const int g0 = (int)(item - row * runs) * ROWS_RUN;
+  const T* src = x + row * ldx;
+  float v[ROWS_RUN][4];
+#pragma unroll
+  for (int i = 0; i < ROWS_RUN; ++i) load4(src, (g0 + i) * FP8_GROUP + 4 * lane, width, vec, v[i]);   // (zeros behind the row's end)
+#pragma unroll
+  for (int i = 0; i < ROWS_RUN; ++i) {
+    const int g = g0 + i, k = g * FP8_GROUP + 4 * lane;
+    if (g >= groups) break;
+    const uint32_t byte = fp8_scale_byte(__reduce_max_sync(0xffffffffu, largest4(v[i])));
+    store4(out + row * ldo, k, width, fp8_pack4(v[i][0], v[i][1], v[i][2], v[i][3], fp8_inverse_scale(byte)));
+    if (lane == 0) scales[row * lds + g] = (uint8_t)byte;
+  }
 }
 
-// A CTA per row: y = (w x) / sqrt(mean(x^2) + eps) in 32 bits, a warp per group.
+// A CTA per row: y = (w x) / sqrt(mean(x^2) + eps) in 32 bits.  Warp i of W takes the groups i, i + W, ...: PER of them, which stay
+// in registers between the sum and the rounding (PER = 0: any number, read twice).
+template <int PER>
 __global__ void rms_norm_rows_kernel(const float* __restrict__ x, const float* __restrict__ w, uint8_t* __restrict__ out, long long ldo,
                                      uint8_t* __restrict__ scales, long long lds, const int* __restrict__ gather, int width, int groups,
                                      float eps, int vec) {
-  __shared__ float scratch[33];
+  __shared__ float part[32];
   pdl_trigger();
   pdl_wait();
-  const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const float* src = x + (size_t)(gather ? gather[row] : row) * width;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const float* src = x + (size_t)(gather ? gather[blockIdx.x] : (int)blockIdx.x) * width;
+  uint8_t* dst = out + (size_t)blockIdx.x * ldo;
+  float v[PER > 0 ? PER : 1][4], f[PER > 0 ? PER : 1][4];
   float sum = 0.f;
-  for (int g = warp; g < groups; g += warps) {
-    float v[4];
-    load4(src, g * FP8_GROUP + 4 * lane, width, vec, v);
-    sum += v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3];
-  }
-  sum = block_sum(sum, scratch);
-  const float inv = 1.f / sqrtf(sum / (float)width + eps);
-  for (int g = warp; g < groups; g += warps) {
-    const int k = g * FP8_GROUP + 4 * lane;
-    float v[4], f[4];
-    load4(src, k, width, vec, v);
-    load4(w, k, width, vec, f);
+  if (PER > 0) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = (f[e] * v[e]) * inv;
-    const uint32_t byte = fp8_scale_byte(__reduce_max_sync(0xffffffffu, largest4(v)));
-    store4(out + (size_t)row * ldo, k, width, fp8_pack4(v[0], v[1], v[2], v[3], fp8_inverse_scale(byte)));
-    if (lane == 0) scales[(size_t)row * lds + g] = (uint8_t)byte;
+    for (int i = 0; i < PER; ++i) load4(src, (warp + i * warps) * FP8_GROUP + 4 * lane, width, vec, v[i]);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) load4(w, (warp + i * warps) * FP8_GROUP + 4 * lane, width, vec, f[i]);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum += v[i][0] * v[i][0] + v[i][1] * v[i][1] + v[i][2] * v[i][2] + v[i][3] * v[i][3];
+  } else {
+    for (int g = warp; g < groups; g += warps) {
+      load4(src, g * FP8_GROUP + 4 * lane, width, vec, v[0]);
+      sum += v[0][0] * v[0][0] + v[0][1] * v[0][1] + v[0][2] * v[0][2] + v[0][3] * v[0][3];
+    }
+  }
+  sum = warp_sum(sum);
+  if (lane == 0) part[warp] = sum;
+  __syncthreads();
+  sum = warp_sum(lane < warps ? part[lane] : 0.f);
+  const float inv = 1.f / sqrtf(sum / (float)width + eps);
+  auto leave = [&](int g, float* y, const float* gain) {
+    const int k = g * FP8_GROUP + 4 * lane;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (gain[e] * y[e]) * inv;
+    const uint32_t byte = fp8_scale_byte(__reduce_max_sync(0xffffffffu, largest4(y)));
+    store4(dst, k, width, fp8_pack4(y[0], y[1], y[2], y[3], fp8_inverse_scale(byte)));
+    if (lane == 0) scales[(size_t)blockIdx.x * lds + g] = (uint8_t)byte;
+  };
+  if (PER > 0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (warp + i * warps < groups) leave(warp + i * warps, v[i], f[i]);
+  } else {
+    for (int g = warp; g < groups; g += warps) {
+      load4(src, g * FP8_GROUP + 4 * lane, width, vec, v[0]);
+      load4(w, g * FP8_GROUP + 4 * lane, width, vec, f[0]);
+      leave(g, v[0], f[0]);
+    }
   }
 }
 
@@ -152,15 +183,16 @@ extern "C" int tllm_quantize_fp8(const QuantizeCall* c) {
   const auto [x, ldx, out, ldo, scales, lds, rows, width, dtype, stream] = *c;
   if (int e = check_rows("quantize_fp8", rows, width, out, ldo, lds)) return e;
   const int groups = (width + FP8_GROUP - 1) / FP8_GROUP;
-  const long long blocks = ((long long)rows * groups + ROWS_THREADS / 32 - 1) / (ROWS_THREADS / 32);
-  TLLM_REQUIRE(blocks < (1ll << 31), "quantize_fp8: %d rows of %d values are too many for one launch", rows, width);
+  const int runs = (groups + ROWS_RUN - 1) / ROWS_RUN;
+  TLLM_REQUIRE((long long)rows * runs < (1ll << 31), "quantize_fp8: %d rows of %d values are too many for one launch", rows, width);
+  const unsigned blocks = ((unsigned)rows * runs + ROWS_THREADS / 32 - 1) / (ROWS_THREADS / 32);
   const int bytes = dtype == TLLM_F32 ? 16 : 8;
   const int vec = (uintptr_t)x % bytes == 0 && ldx % 4 == 0;
   cudaStream_t s = (cudaStream_t)stream;
   if (dtype == TLLM_F32)
-    TLLM_LAUNCH("quantize_fp8", quantize_rows_kernel<float>, (unsigned)blocks, ROWS_THREADS, 0, s, (const float*)x, ldx, (uint8_t*)out, ldo, (uint8_t*)scales, lds, rows, width, groups, vec);
+    TLLM_LAUNCH("quantize_fp8", quantize_rows_kernel<float>, blocks, ROWS_THREADS, 0, s, (const float*)x, ldx, (uint8_t*)out, ldo, (uint8_t*)scales, lds, rows, width, groups, runs, vec);
   else
-    TLLM_LAUNCH("quantize_fp8", quantize_rows_kernel<__nv_bfloat16>, (unsigned)blocks, ROWS_THREADS, 0, s, (const __nv_bfloat16*)x, ldx, (uint8_t*)out, ldo, (uint8_t*)scales, lds, rows, width, groups, vec);
+    TLLM_LAUNCH("quantize_fp8", quantize_rows_kernel<__nv_bfloat16>, blocks, ROWS_THREADS, 0, s, (const __nv_bfloat16*)x, ldx, (uint8_t*)out, ldo, (uint8_t*)scales, lds, rows, width, groups, runs, vec);
   return TLLM_OK;
 }
 
@@ -170,8 +202,13 @@ extern "C" int tllm_rms_norm_fp8(const RmsNormCall* c) {
   if (int e = check_rows("rms_norm_fp8", rows, width, out, ldo, lds)) return e;
   const int groups = (width + FP8_GROUP - 1) / FP8_GROUP;
   const int vec = (uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0 && width % 4 == 0;
-  const int threads = groups >= 16 ? 512 : (groups >= 8 ? 256 : 128);
-  TLLM_LAUNCH("rms_norm_fp8", rms_norm_rows_kernel, rows, threads, 0, (cudaStream_t)stream, x, w, (uint8_t*)out, ldo, (uint8_t*)scales, lds, rows_idx, width, groups, eps, vec);
+  // Few rows leave most SMs idle: a warp per group is the shortest way through a row.  Many rows: eight groups per warp, so that more
+  // rows fit an SM.
+  const int per = rows <= 296 ? (groups <= 16 ? 1 : groups <= 32 ? 2 : groups <= 64 ? 4 : 8) : 8;
+  const int warps = min(32, max(1, (groups + per - 1) / per));
+  auto kern = warps * per < groups ? rms_norm_rows_kernel<0> : per == 1 ? rms_norm_rows_kernel<1> : per == 2 ? rms_norm_rows_kernel<2>
+              : per == 4 ? rms_norm_rows_kernel<4> : rms_norm_rows_kernel<8>;
+  TLLM_LAUNCH("rms_norm_fp8", kern, rows, 32 * warps, 0, (cudaStream_t)stream, x, w, (uint8_t*)out, ldo, (uint8_t*)scales, lds, rows_idx, width, groups, eps, vec);
   return TLLM_OK;
 }
 
