@@ -21,20 +21,19 @@ __device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t largest) {
   const int byte = (int)((largest + 0x1FFFFFu) >> 23) - 8;   // a mantissa above 1.75 carries into the exponent
   return largest == 0u ? 127u : (uint32_t)max(byte, 1);
 }
-// 1 / scale; 0 stands for "all values become 0"
-__device__ __forceinline__ float fp8_inverse_scale(uint32_t byte) { return byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23); }
+// 1 / scale (whatever for NaN: fp8_pack4 leaves zeros there)
+__device__ __forceinline__ float fp8_inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 // The scale an e8m0 byte stands for: 2^(byte - 127), 255 NaN.
 __device__ __forceinline__ float fp8_scale(uint32_t byte) {
   return byte == 255u ? __uint_as_float(0x7FC00000u) : byte == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
 }
 __device__ __forceinline__ uint32_t fp8_abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-// four values to four e4m3 bytes, the first in the lowest
-__device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d, float inverse) {
-  if (inverse == 0.f) return 0u;
+// four values over the scale 2^(byte - 127) as four e4m3 bytes, the first in the lowest; zeros where the scale is NaN
+__device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d, float inverse, uint32_t byte) {
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a * inverse, b * inverse), __NV_SATFINITE, __NV_E4M3);
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c * inverse, d * inverse), __NV_SATFINITE, __NV_E4M3);
-  return lo | (hi << 16);
+  return byte == 255u ? 0u : __byte_perm(lo, hi, 0x5410);
 }
 
 }  // namespace tllm

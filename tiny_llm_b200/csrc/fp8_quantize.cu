@@ -5,6 +5,9 @@
 //   * weights [N, K]: one float32 scale per block of 128 x 128.
 // All are bound by memory: every value is read once (the norm's rows a second time where they do not fit the registers) and
 // leaves as one byte.
+#include <climits>
+#include <type_traits>
+
 #include "fp8.cuh"
 
 TLLM_DEFINE_LAST_ERROR
@@ -44,12 +47,25 @@ __device__ __forceinline__ void store4(uint8_t* dst, int k, int width, uint32_t 
 __device__ __forceinline__ uint32_t largest4(const float* v) {
   return max(max(fp8_abs_bits(v[0]), fp8_abs_bits(v[1])), max(fp8_abs_bits(v[2]), fp8_abs_bits(v[3])));
 }
+__device__ __forceinline__ void unpack2(uint32_t u, float& a, float& b) { a = __uint_as_float(u << 16); b = __uint_as_float(u & 0xFFFF0000u); }
+
+// A warp's group of 128, four values per lane, to `dst` + k; returns the scale's byte.
+__device__ __forceinline__ uint32_t leave_group(const float* v, uint8_t* dst, int k, int width) {
+  const uint32_t byte = fp8_scale_byte(__reduce_max_sync(0xffffffffu, largest4(v)));
+  store4(dst, k, width, fp8_pack4(v[0], v[1], v[2], v[3], fp8_inverse_scale(byte), byte));
+  return byte;
+}
 
 constexpr int ROWS_THREADS = 256;
 
-// A warp per row and run of four groups: four values per lane and group, the four loads in flight together.
-constexpr int ROWS_RUN = 4;
-template <typename T>
+// A warp per row and run of groups, all of the run's loads in flight together: four groups of float32, four values per lane, or
+// eight of bfloat16, eight values per lane and half a warp per group.  With 16-byte loads and no checks inside a run the kernel
+// issues 25 instructions per group of bfloat16 instead of 86 and is bound by memory.
+// (Few rows: runs a quarter as long, so that four times the warps share the work.)
+template <typename T> struct Run { static constexpr int LONG = 4, SHORT = 1; };
+template <> struct Run<__nv_bfloat16> { static constexpr int LONG = 8, SHORT = 2; };
+
+template <typename T, int GROUPS>
 __global__ void __launch_bounds__(ROWS_THREADS)
 quantize_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ out, long long ldo,
                      uint8_t* __restrict__ scales, long long lds, int rows, int width, int groups, int runs, int vec) {
@@ -59,24 +75,63 @@ quantize_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict
   const unsigned item = blockIdx.x * (ROWS_THREADS / 32) + (threadIdx.x >> 5);
   const unsigned row = item / (unsigned)runs;
   if (row >= (unsigned)rows) return;
-  const int g0 = (int)(item - row * runs) * ROWS_RUN;
+  const int g0 = (int)(item - row * runs) * GROUPS;
   const T* src = x + row * ldx;
-  float v[ROWS_RUN][4];
+  uint8_t* dst = out + row * ldo;
+  uint32_t mine = 0u;      // lane i keeps the byte of the run's group i
+  if (vec && (g0 + GROUPS) * FP8_GROUP <= width) {
+    if constexpr (sizeof(T) == 2) {
+      uint4 u[GROUPS / 2];
 #pragma unroll
-  for (int i = 0; i < ROWS_RUN; ++i) load4(src, (g0 + i) * FP8_GROUP + 4 * lane, width, vec, v[i]);   // (zeros behind the row's end)
+      for (int i = 0; i < GROUPS / 2; ++i) u[i] = *reinterpret_cast<const uint4*>(src + (g0 + 2 * i) * FP8_GROUP + 8 * lane);
 #pragma unroll
-  for (int i = 0; i < ROWS_RUN; ++i) {
-    const int g = g0 + i, k = g * FP8_GROUP + 4 * lane;
-    if (g >= groups) break;
-    const uint32_t byte = fp8_scale_byte(__reduce_max_sync(0xffffffffu, largest4(v[i])));
-    store4(out + row * ldo, k, width, fp8_pack4(v[i][0], v[i][1], v[i][2], v[i][3], fp8_inverse_scale(byte)));
-    if (lane == 0) scales[row * lds + g] = (uint8_t)byte;
+      for (int i = 0; i < GROUPS / 2; ++i) {
+        // magnitudes of bfloat16 are ordered as 16-bit integers, two to a word
+        uint32_t most = __vmaxu2(__vmaxu2(u[i].x & 0x7FFF7FFFu, u[i].y & 0x7FFF7FFFu), __vmaxu2(u[i].z & 0x7FFF7FFFu, u[i].w & 0x7FFF7FFFu));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const uint32_t byte = fp8_scale_byte(max(most << 16, most & 0xFFFF0000u));
+        const float inverse = fp8_inverse_scale(byte);
+        float v[8];
+        unpack2(u[i].x, v[0], v[1]); unpack2(u[i].y, v[2], v[3]); unpack2(u[i].z, v[4], v[5]); unpack2(u[i].w, v[6], v[7]);
+        *reinterpret_cast<uint2*>(dst + (g0 + 2 * i) * FP8_GROUP + 8 * lane) =
+            make_uint2(fp8_pack4(v[0], v[1], v[2], v[3], inverse, byte), fp8_pack4(v[4], v[5], v[6], v[7], inverse, byte));
+        const uint32_t first = __shfl_sync(0xffffffffu, byte, 0), second = __shfl_sync(0xffffffffu, byte, 16);
+        mine = lane == 2 * i ? first : lane == 2 * i + 1 ? second : mine;
+      }
+    } else {
+      float4 f[GROUPS];
+#pragma unroll
+      for (int i = 0; i < GROUPS; ++i) f[i] = *reinterpret_cast<const float4*>(src + (g0 + i) * FP8_GROUP + 4 * lane);
+#pragma unroll
+      for (int i = 0; i < GROUPS; ++i) {
+        const float v[4] = {f[i].x, f[i].y, f[i].z, f[i].w};
+        const uint32_t byte = leave_group(v, dst, (g0 + i) * FP8_GROUP + 4 * lane, width);
+        mine = lane == i ? byte : mine;
+      }
+    }
+  } else {
+    constexpr int HALF = GROUPS < 4 ? GROUPS : 4;
+    const bool vec4 = (reinterpret_cast<uintptr_t>(src) & (4 * sizeof(T) - 1)) == 0;
+#pragma unroll
+    for (int h = 0; h < GROUPS; h += HALF) {
+      float v[HALF][4];
+#pragma unroll
+      for (int i = 0; i < HALF; ++i) load4(src, (g0 + h + i) * FP8_GROUP + 4 * lane, width, vec4, v[i]);   // (zeros behind the row's end)
+#pragma unroll
+      for (int i = 0; i < HALF; ++i) {
+        if (g0 + h + i >= groups) break;
+        const uint32_t byte = leave_group(v[i], dst, (g0 + h + i) * FP8_GROUP + 4 * lane, width);
+        mine = lane == h + i ? byte : mine;
+      }
+    }
   }
+  if (lane < GROUPS && g0 + lane < groups) scales[row * lds + g0 + lane] = (uint8_t)mine;
 }
 
 // A CTA per row: y = (w x) / sqrt(mean(x^2) + eps) in 32 bits.  Warp i of W takes the groups i, i + W, ...: PER of them, which stay
-// in registers between the sum and the rounding (PER = 0: any number, read twice).
-template <int PER>
+// in registers between the sum and the rounding (PER = 0: any number, read twice).  FULL: the row is whole groups, on 16 bytes.
+template <int PER, bool FULL>
 __global__ void rms_norm_rows_kernel(const float* __restrict__ x, const float* __restrict__ w, uint8_t* __restrict__ out, long long ldo,
                                      uint8_t* __restrict__ scales, long long lds, const int* __restrict__ gather, int width, int groups,
                                      float eps, int vec) {
@@ -86,18 +141,27 @@ __global__ void rms_norm_rows_kernel(const float* __restrict__ x, const float* _
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const float* src = x + (size_t)(gather ? gather[blockIdx.x] : (int)blockIdx.x) * width;
   uint8_t* dst = out + (size_t)blockIdx.x * ldo;
-  float v[PER > 0 ? PER : 1][4], f[PER > 0 ? PER : 1][4];
-  float sum = 0.f;
+  auto load = [&](const float* from, int g, float* v) {
+    if (FULL) {
+      const float4 f = g < groups ? *reinterpret_cast<const float4*>(from + g * FP8_GROUP + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    } else {
+      load4(from, g * FP8_GROUP + 4 * lane, width, vec, v);
+    }
+  };
+  // the gains come in batches, the first while the row's sum is under way
+  constexpr int BATCH = PER >= 4 ? 4 : PER > 0 ? PER : 1;
+  float v[PER > 0 ? PER : 1][4], gain[BATCH][4], sum = 0.f;
   if (PER > 0) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) load4(src, (warp + i * warps) * FP8_GROUP + 4 * lane, width, vec, v[i]);
+    for (int i = 0; i < PER; ++i) load(src, warp + i * warps, v[i]);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) load4(w, (warp + i * warps) * FP8_GROUP + 4 * lane, width, vec, f[i]);
+    for (int i = 0; i < BATCH; ++i) load(w, warp + i * warps, gain[i]);
 #pragma unroll
     for (int i = 0; i < PER; ++i) sum += v[i][0] * v[i][0] + v[i][1] * v[i][1] + v[i][2] * v[i][2] + v[i][3] * v[i][3];
   } else {
     for (int g = warp; g < groups; g += warps) {
-      load4(src, g * FP8_GROUP + 4 * lane, width, vec, v[0]);
+      load(src, g, v[0]);
       sum += v[0][0] * v[0][0] + v[0][1] * v[0][1] + v[0][2] * v[0][2] + v[0][3] * v[0][3];
     }
   }
@@ -106,64 +170,93 @@ __global__ void rms_norm_rows_kernel(const float* __restrict__ x, const float* _
   __syncthreads();
   sum = warp_sum(lane < warps ? part[lane] : 0.f);
   const float inv = 1.f / sqrtf(sum / (float)width + eps);
-  auto leave = [&](int g, float* y, const float* gain) {
-    const int k = g * FP8_GROUP + 4 * lane;
+  auto leave = [&](int g, float* y, const float* f) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = (gain[e] * y[e]) * inv;
-    const uint32_t byte = fp8_scale_byte(__reduce_max_sync(0xffffffffu, largest4(y)));
-    store4(dst, k, width, fp8_pack4(y[0], y[1], y[2], y[3], fp8_inverse_scale(byte)));
+    for (int e = 0; e < 4; ++e) y[e] = (f[e] * y[e]) * inv;
+    const uint32_t byte = leave_group(y, dst, g * FP8_GROUP + 4 * lane, FULL ? INT_MAX : width);
     if (lane == 0) scales[(size_t)blockIdx.x * lds + g] = (uint8_t)byte;
   };
   if (PER > 0) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (warp + i * warps < groups) leave(warp + i * warps, v[i], f[i]);
+    for (int h = 0; h < PER; h += BATCH) {
+      if (h > 0) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) load(w, warp + (h + i) * warps, gain[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i)
+        if (warp + (h + i) * warps < groups) leave(warp + (h + i) * warps, v[h + i], gain[i]);
+    }
   } else {
     for (int g = warp; g < groups; g += warps) {
-      load4(src, g * FP8_GROUP + 4 * lane, width, vec, v[0]);
-      load4(w, g * FP8_GROUP + 4 * lane, width, vec, f[0]);
-      leave(g, v[0], f[0]);
+      load(src, g, v[0]);
+      load(w, g, gain[0]);
+      leave(g, v[0], gain[0]);
     }
   }
 }
 
 constexpr int WEIGHT_THREADS = 512;
 
-// A CTA per block of 128 x 128, which stays in registers between the search for its largest magnitude and the rounding.  The
-// products may begin to read a weight while earlier launches still run, so this kernel never lets the next one start early.
+// four values of a lane as they came
+template <typename T> struct Held { float4 v; };
+template <> struct Held<__nv_bfloat16> { uint2 v; };
+__device__ __forceinline__ void give(const Held<float>& h, float* v) { v[0] = h.v.x; v[1] = h.v.y; v[2] = h.v.z; v[3] = h.v.w; }
+__device__ __forceinline__ void give(const Held<__nv_bfloat16>& h, float* v) { unpack2(h.v.x, v[0], v[1]); unpack2(h.v.y, v[2], v[3]); }
+__device__ __forceinline__ void take(Held<float>& h, const float* src, int k, int width, bool vec) {
+  if (vec && k + 4 <= width) { h.v = *reinterpret_cast<const float4*>(src + k); return; }
+  float v[4];
+  load4(src, k, width, false, v);
+  h.v = make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void take(Held<__nv_bfloat16>& h, const __nv_bfloat16* src, int k, int width, bool vec) {
+  if (vec && k + 4 <= width) { h.v = *reinterpret_cast<const uint2*>(src + k); return; }
+  float v[4];
+  load4(src, k, width, false, v);
+  h.v = make_uint2((__float_as_uint(v[0]) >> 16) | __float_as_uint(v[1]), (__float_as_uint(v[2]) >> 16) | __float_as_uint(v[3]));
+}
+
+// A CTA per block of 128 x 128, which stays in registers (bfloat16 as it came) between the search for its largest magnitude and the
+// rounding.  The products may begin to read a weight while earlier launches still run, so this kernel never lets the next one start
+// early, and its values are in memory before it ends.
 template <typename T>
-__global__ void __launch_bounds__(WEIGHT_THREADS)
+__global__ void __launch_bounds__(WEIGHT_THREADS, 3)
 quantize_weight_kernel(const T* __restrict__ w, long long ldw, uint8_t* __restrict__ out, long long ldo, float* __restrict__ scales,
                        int rows, int width, int groups, int vec) {
   constexpr int WARPS = WEIGHT_THREADS / 32, PER = FP8_GROUP / WARPS;
   __shared__ uint32_t most[WARPS];
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int k = blockIdx.x * FP8_GROUP + 4 * lane, n0 = blockIdx.y * FP8_GROUP;
-  float v[PER][4];
-  uint32_t largest = 0u;
+  const int k = blockIdx.x * FP8_GROUP + 4 * lane, n0 = blockIdx.y * FP8_GROUP + warp;
+  Held<T> held[PER];
+  const T* src = w + (long long)n0 * ldw;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int n = n0 + i * WARPS + warp;
-    if (n < rows) load4(w + n * ldw, k, width, vec, v[i]);
-    else v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
+    if (n0 + i * WARPS < rows) take(held[i], src + (long long)i * WARPS * ldw, k, width, vec);
+    else held[i].v = {};
   }
+  uint32_t largest = 0u;
+  float v[4];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) largest = max(largest, largest4(v[i]));
+  for (int i = 0; i < PER; ++i) {
+    give(held[i], v);
+    largest = max(largest, largest4(v));
+  }
   largest = __reduce_max_sync(0xffffffffu, largest);
   if (lane == 0) most[warp] = largest;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < WARPS; ++i) largest = max(largest, most[i]);
+  largest = __reduce_max_sync(0xffffffffu, most[lane % WARPS]);
   const uint32_t byte = fp8_scale_byte(largest);
   const float inverse = fp8_inverse_scale(byte);
+  uint8_t* dst = out + (long long)n0 * ldo;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int n = n0 + i * WARPS + warp;
-    if (n < rows) store4(out + n * ldo, k, width, fp8_pack4(v[i][0], v[i][1], v[i][2], v[i][3], inverse));
+    give(held[i], v);
+    if (n0 + i * WARPS < rows) store4(dst + (long long)i * WARPS * ldo, k, width, fp8_pack4(v[0], v[1], v[2], v[3], inverse, byte));
   }
   if (threadIdx.x == 0) scales[(size_t)blockIdx.y * groups + blockIdx.x] = fp8_scale(byte);
-  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) __threadfence();
 }
 
 static int check_rows(const char* name, int rows, int width, const void* out, long long ldo, long long lds) {
@@ -183,17 +276,20 @@ extern "C" int tllm_quantize_fp8(const QuantizeCall* c) {
   const auto [x, ldx, out, ldo, scales, lds, rows, width, dtype, stream] = *c;
   if (int e = check_rows("quantize_fp8", rows, width, out, ldo, lds)) return e;
   const int groups = (width + FP8_GROUP - 1) / FP8_GROUP;
-  const int runs = (groups + ROWS_RUN - 1) / ROWS_RUN;
+  const bool few = (long long)rows * groups <= 148 * 32;
+  const int run = dtype == TLLM_F32 ? (few ? Run<float>::SHORT : Run<float>::LONG) : (few ? Run<__nv_bfloat16>::SHORT : Run<__nv_bfloat16>::LONG);
+  const int runs = (groups + run - 1) / run;
   TLLM_REQUIRE((long long)rows * runs < (1ll << 31), "quantize_fp8: %d rows of %d values are too many for one launch", rows, width);
   const unsigned blocks = ((unsigned)rows * runs + ROWS_THREADS / 32 - 1) / (ROWS_THREADS / 32);
-  const int bytes = dtype == TLLM_F32 ? 16 : 8;
-  const int vec = (uintptr_t)x % bytes == 0 && ldx % 4 == 0;
+  const int vec = (uintptr_t)x % 16 == 0 && ldx % (dtype == TLLM_F32 ? 4 : 8) == 0;
   cudaStream_t s = (cudaStream_t)stream;
-  if (dtype == TLLM_F32)
-    TLLM_LAUNCH("quantize_fp8", quantize_rows_kernel<float>, blocks, ROWS_THREADS, 0, s, (const float*)x, ldx, (uint8_t*)out, ldo, (uint8_t*)scales, lds, rows, width, groups, runs, vec);
-  else
-    TLLM_LAUNCH("quantize_fp8", quantize_rows_kernel<__nv_bfloat16>, blocks, ROWS_THREADS, 0, s, (const __nv_bfloat16*)x, ldx, (uint8_t*)out, ldo, (uint8_t*)scales, lds, rows, width, groups, runs, vec);
-  return TLLM_OK;
+  auto launch = [&](auto zero, auto kern) -> int {
+    using T = decltype(zero);
+    TLLM_LAUNCH("quantize_fp8", kern, blocks, ROWS_THREADS, 0, s, (const T*)x, ldx, (uint8_t*)out, ldo, (uint8_t*)scales, lds, rows, width, groups, runs, vec);
+    return TLLM_OK;
+  };
+  if (dtype == TLLM_F32) return launch(0.f, few ? quantize_rows_kernel<float, Run<float>::SHORT> : quantize_rows_kernel<float, Run<float>::LONG>);
+  return launch(__nv_bfloat16(), few ? quantize_rows_kernel<__nv_bfloat16, Run<__nv_bfloat16>::SHORT> : quantize_rows_kernel<__nv_bfloat16, Run<__nv_bfloat16>::LONG>);
 }
 
 struct RmsNormCall { const float *x, *w; void* out; long long ldo; void* scales; long long lds; const int* rows_idx; int rows, width; float eps; void* stream; };
@@ -206,8 +302,13 @@ extern "C" int tllm_rms_norm_fp8(const RmsNormCall* c) {
   // rows fit an SM.
   const int per = rows <= 296 ? (groups <= 16 ? 1 : groups <= 32 ? 2 : groups <= 64 ? 4 : 8) : 8;
   const int warps = min(32, max(1, (groups + per - 1) / per));
-  auto kern = warps * per < groups ? rms_norm_rows_kernel<0> : per == 1 ? rms_norm_rows_kernel<1> : per == 2 ? rms_norm_rows_kernel<2>
-              : per == 4 ? rms_norm_rows_kernel<4> : rms_norm_rows_kernel<8>;
+  const bool full = vec && width % FP8_GROUP == 0;
+  auto pick = [&](auto whole) {
+    constexpr bool F = decltype(whole)::value;
+    return warps * per < groups ? rms_norm_rows_kernel<0, F> : per == 1 ? rms_norm_rows_kernel<1, F> : per == 2 ? rms_norm_rows_kernel<2, F>
+           : per == 4 ? rms_norm_rows_kernel<4, F> : rms_norm_rows_kernel<8, F>;
+  };
+  auto kern = full ? pick(std::true_type()) : pick(std::false_type());
   TLLM_LAUNCH("rms_norm_fp8", kern, rows, 32 * warps, 0, (cudaStream_t)stream, x, w, (uint8_t*)out, ldo, (uint8_t*)scales, lds, rows_idx, width, groups, eps, vec);
   return TLLM_OK;
 }

@@ -267,10 +267,10 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 #pragma unroll
             for (int j = 0; j < 64; j += 16) {
               uint4 pk;
-              pk.x = fp8_pack4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3], inverse);
-              pk.y = fp8_pack4(acc[j + 4], acc[j + 5], acc[j + 6], acc[j + 7], inverse);
-              pk.z = fp8_pack4(acc[j + 8], acc[j + 9], acc[j + 10], acc[j + 11], inverse);
-              pk.w = fp8_pack4(acc[j + 12], acc[j + 13], acc[j + 14], acc[j + 15], inverse);
+              pk.x = fp8_pack4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3], inverse, byte);
+              pk.y = fp8_pack4(acc[j + 4], acc[j + 5], acc[j + 6], acc[j + 7], inverse, byte);
+              pk.z = fp8_pack4(acc[j + 8], acc[j + 9], acc[j + 10], acc[j + 11], inverse, byte);
+              pk.w = fp8_pack4(acc[j + 12], acc[j + 13], acc[j + 14], acc[j + 15], inverse, byte);
               if (n + j + 16 <= p.n) {
                 *reinterpret_cast<uint4*>(dst + j) = pk;
               } else {
