@@ -77,6 +77,18 @@ __device__ __forceinline__ bool sums_all(bool ok) {
       : "=r"(r) : "r"((uint32_t)ok), "n"(32 * SUM_WARPS) : "memory");
   return r != 0;
 }
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// four floats at byte address `addr` of this CTA's shared memory, read from the CTA of rank `rank` in the cluster
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr, uint32_t rank) {
+  uint32_t remote;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
+  return v;
+}
 
 template <int BN, int STAGES>
 struct Smem {
@@ -290,6 +302,235 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   if (warp == 1) tmem_dealloc(tmem_base, 2 * BN);
 }
 
+// ---------------------------------------------------------------- few rows
+// Up to 128 rows of A: the weight is the 128-row operand, the rows of A are the BN columns, and K is cut into slices so that every
+// SM streams weights; such a product is bound by reading them once.  The slices of one tile are a thread-block cluster: every CTA
+// adds its groups up in registers (a thread per weight row), leaves the sums in its shared memory, and after a cluster barrier the
+// CTAs share the tile's tokens, a warp per token: it adds the slices over the peers' shared memory in a fixed order, four weight rows
+// per lane, and stores 128 neighbouring columns.  Gated: a CTA has the gate tile and the up tile beside it, two accumulators and four
+// warps for each; the 128 columns that a warp stores are one group of the product behind.
+constexpr int FEW_CHUNK = 16;    // groups whose scales (of the row times of the block) are laid out in shared memory at a time
+
+template <int BN, int STAGES, bool GATED>
+struct FewSmem {
+  static constexpr int TILES = GATED ? 2 : 1, W_BYTES = TILES * 128 * BK, A_BYTES = BN * BK, STAGE_BYTES = W_BYTES + A_BYTES;
+  static constexpr int SCALE_OFFSET = STAGES * STAGE_BYTES;
+  static constexpr int BAR_OFFSET = SCALE_OFFSET + TILES * FEW_CHUNK * BN * 4;
+  static constexpr int TOTAL = BAR_OFFSET + (2 * STAGES + 4) * 8 + 16 + 1024;
+  static_assert(TILES * BN * 128 * 4 <= STAGES * STAGE_BYTES, "the sums are left where the stages were");
+};
+
+struct FewArgs {
+  int slices, per_slice;       // slices of K (the cluster), groups per slice (the last may have fewer, or none)
+};
+
+template <int BN, int STAGES, bool GATED>
+__global__ void __launch_bounds__(GATED ? 320 : 192, (FewSmem<BN, STAGES, GATED>::TOTAL <= 113 * 1024) ? 2 : 1)
+linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const Fp8Args p, const FewArgs f, int* __restrict__ status) {
+  using L = FewSmem<BN, STAGES, GATED>;
+  constexpr int TILES = L::TILES, FEW_SUM_WARPS = 4 * TILES, WARPS = 2 + FEW_SUM_WARPS;
+  constexpr uint32_t ACC_COLS = TILES * BN, TMEM_COLS = 2 * ACC_COLS < 32 ? 32 : 2 * ACC_COLS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  float* scale = reinterpret_cast<float*>(smem + L::SCALE_OFFSET);     // [TILES][FEW_CHUNK][BN]
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::BAR_OFFSET);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* acc_full = empty_bar + STAGES;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  float* parked = reinterpret_cast<float*>(smem);                      // [TILES][BN tokens][128 weight rows] once the stages are done with
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int m0 = blockIdx.x * BN, tile = blockIdx.y, rank = blockIdx.z;
+  const int g_begin = min(p.groups, rank * f.per_slice), n_g = min(p.groups, g_begin + f.per_slice) - g_begin;
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_map(&map_w); tma_prefetch_map(&map_a);
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], FEW_SUM_WARPS); }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  // the weight depends on no earlier kernel: the first stages are asked for before this grid waits for its predecessors
+  pdl_trigger();
+  const int n_pre = min(n_g, STAGES);
+  auto load_weight = [&](int i, uint64_t policy) {
+    const int s = i % STAGES;
+    mbar_expect_tx(&full_bar[s], L::STAGE_BYTES);
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+      tma_load_2d_hint(smem + s * L::STAGE_BYTES + t * 128 * BK, &map_w, (g_begin + i) * BK, (tile * TILES + t) * 128, &full_bar[s], policy);
+  };
+  // (read once, unless several tiles of rows share it)
+  const uint64_t policy = l2_evict_first_policy();
+  if (warp == 0 && lane == 0)
+    for (int i = 0; i < n_pre; ++i) load_weight(i, policy);
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------- TMA producer
+      int i = 0;
+      for (; i < n_g; ++i) {
+        const int s = i % STAGES;
+        if (i >= n_pre) {
+          if (!mbar_wait(&empty_bar[s], ((i / STAGES) & 1) ^ 1, abort_flag)) { *abort_flag = 1; atomicExch(status, ERR_F8_PRODUCER); break; }
+          load_weight(i, policy);
+        }
+        tma_load_2d(smem + s * L::STAGE_BYTES + L::W_BYTES, &map_a, (g_begin + i) * BK, m0, &full_bar[s]);
+      }
+      mbar_drain(full_bar, STAGES, i);
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer
+    const uint32_t idesc = instr_desc_e4m3(128, BN);
+    const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
+    const uint32_t lo0 = smem_desc_sw128_lo(smem_u32(smem));
+    bool ok = true;
+    for (int i = 0; i < n_g; ++i) {
+      const int s = i % STAGES, buf = i & 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((i >> 1) & 1) ^ 1, abort_flag) && mbar_wait(&full_bar[s], (i / STAGES) & 1, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t w_lo = lo0 + s * (L::STAGE_BYTES >> 4), a_lo = w_lo + (L::W_BYTES >> 4);
+      if (elect_one()) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k)
+            umma_fp8_lo(tmem_u + buf * ACC_COLS + t * BN, w_lo + (t * 128 * BK >> 4) + (k * UMMA_K >> 4), a_lo + (k * UMMA_K >> 4), idesc, k > 0 ? 1u : 0u);
+        umma_commit(&empty_bar[s]);
+        umma_commit(&acc_full[buf]);
+      }
+      __syncwarp();
+    }
+    if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_MMA); }
+  } else {
+    // ---------------- sums: warp w reads tensor-memory lanes [32 (w % 4), +32) of its tile's accumulator
+    const int quad = warp & 3, part = GATED ? (warp - 2) >> 2 : 0, thread = threadIdx.x - 64;
+    const int row = quad * 32 + lane;
+    float acc[BN];
+#pragma unroll
+    for (int j = 0; j < BN; ++j) acc[j] = 0.f;
+    bool ok = true;
+    for (int i0 = 0; i0 < n_g; i0 += FEW_CHUNK) {
+      const int n = min(FEW_CHUNK, n_g - i0);
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * FEW_SUM_WARPS) : "memory");     // the chunk before has been read
+      for (int e = thread; e < FEW_CHUNK * BN; e += 32 * FEW_SUM_WARPS) {
+        const int g = e % FEW_CHUNK, j = e / FEW_CHUNK;
+        const float a = g < n && m0 + j < p.m ? fp8_scale(p.a_scales[(long long)(m0 + j) * p.lda_s + g_begin + i0 + g]) : 0.f;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+          scale[(t * FEW_CHUNK + g) * BN + j] = g < n ? a * p.w_scales[(long long)(tile * TILES + t) * p.groups + g_begin + i0 + g] : 0.f;
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * FEW_SUM_WARPS) : "memory");
+      for (int g = 0; g < n && ok; ++g) {
+        const int i = i0 + g, buf = i & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (i >> 1) & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t taddr = tmem_base + buf * ACC_COLS + part * BN + ((uint32_t)(quad * 32) << 16);
+        const float4* sc = reinterpret_cast<const float4*>(scale + (part * FEW_CHUNK + g) * BN);
+#pragma unroll
+        for (int c = 0; c < BN; c += 16) {
+          float v[16];
+          tmem_ld16(taddr + c, v);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float4 s4 = sc[c / 4 + j];
+            acc[c + 4 * j] = fmaf(v[4 * j], s4.x, acc[c + 4 * j]);
+            acc[c + 4 * j + 1] = fmaf(v[4 * j + 1], s4.y, acc[c + 4 * j + 1]);
+            acc[c + 4 * j + 2] = fmaf(v[4 * j + 2], s4.z, acc[c + 4 * j + 2]);
+            acc[c + 4 * j + 3] = fmaf(v[4 * j + 3], s4.w, acc[c + 4 * j + 3]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      }
+    }
+    if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_SUMS); }
+    // the last accumulator is there, so every product has read its stage: the stages are free
+    float* mine = parked + part * BN * 128 + row;
+#pragma unroll
+    for (int j = 0; j < BN; ++j) mine[j * 128] = acc[j];
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
+
+  if (f.slices > 1) cluster_sync_all();
+  const uint32_t base = smem_u32(parked);
+  const int tokens = min(BN, p.m - m0);
+  for (int j = rank + f.slices * warp; j < tokens; j += f.slices * WARPS) {
+    const int m = m0 + j, n = tile * 128 + 4 * lane;
+    float4 part[TILES][8];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+      for (int z = 0; z < 8; ++z)
+        if (z < f.slices) part[t][z] = ld_cluster_f32x4(base + (uint32_t)((t * BN + j) * 128 + 4 * lane) * 4u, z);
+    float sum[TILES][4];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      sum[t][0] = sum[t][1] = sum[t][2] = sum[t][3] = 0.f;
+#pragma unroll
+      for (int z = 0; z < 8; ++z)
+        if (z < f.slices) { sum[t][0] += part[t][z].x; sum[t][1] += part[t][z].y; sum[t][2] += part[t][z].z; sum[t][3] += part[t][z].w; }
+    }
+    if (GATED) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[0][e] = n + e < p.n ? gate_f(sum[0][e], sum[TILES - 1][e], p.act, p.limit) : 0.f;
+    }
+    if (GATED && p.mode == OUT_FP8) {
+      const uint32_t byte = fp8_scale_byte(__reduce_max_sync(0xffffffffu, max(max(fp8_abs_bits(sum[0][0]), fp8_abs_bits(sum[0][1])),
+                                                                              max(fp8_abs_bits(sum[0][2]), fp8_abs_bits(sum[0][3])))));
+      const uint32_t packed = fp8_pack4(sum[0][0], sum[0][1], sum[0][2], sum[0][3], fp8_inverse_scale(byte), byte);
+      uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + (size_t)m * p.ldo + n;
+      if (lane == 0) p.out_scales[(size_t)m * p.ldo_s + tile] = (uint8_t)byte;
+      if (n + 4 <= p.n) {
+        *reinterpret_cast<uint32_t*>(dst) = packed;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < p.n) dst[e] = (uint8_t)(packed >> (8 * e));
+      }
+    } else if (GATED || p.mode == OUT_BF16) {
+      __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + (size_t)m * p.ldo + n;
+      if (n + 4 <= p.n && p.vec_out) {
+        uint2 pk;
+        reinterpret_cast<__nv_bfloat162*>(&pk)[0] = __floats2bfloat162_rn(sum[0][0], sum[0][1]);
+        reinterpret_cast<__nv_bfloat162*>(&pk)[1] = __floats2bfloat162_rn(sum[0][2], sum[0][3]);
+        *reinterpret_cast<uint2*>(dst) = pk;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < p.n) dst[e] = __float2bfloat16_rn(sum[0][e]);
+      }
+    } else {
+      float* dst = reinterpret_cast<float*>(p.out) + (size_t)m * p.ldo + n;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < p.n) sum[0][e] += p.mode == OUT_ADD ? dst[e] : 0.f;
+      if (n + 4 <= p.n && p.vec_out) {
+        *reinterpret_cast<float4*>(dst) = make_float4(sum[0][0], sum[0][1], sum[0][2], sum[0][3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < p.n) dst[e] = sum[0][e];
+      }
+    }
+  }
+  if (f.slices > 1) cluster_sync_all();   // no CTA leaves while a peer still reads its shared memory
+}
+
 // ---------------------------------------------------------------- host side
 // A 2-D tensor of bytes [rows, k] with row stride ld, tiled in boxes of box_rows x 128.
 static bool make_map(CUtensorMap* map, const void* ptr, int rows, int k, long long ld, int box_rows) {
@@ -330,6 +571,39 @@ static int launch_tiles(const Fp8Args& p, const void* a, long long lda, const vo
   return TLLM_OK;
 }
 
+template <int BN, int STAGES, bool GATED>
+static int launch_few(const Fp8Args& p, const void* a, long long lda, const void* w, long long ldw, int w_rows, int k, int* status, cudaStream_t s) {
+  using L = FewSmem<BN, STAGES, GATED>;
+  auto kern = linear_fp8_few_kernel<BN, STAGES, GATED>;
+  TLLM_RESERVE_SMEM("linear_fp8", L::TOTAL, kern);
+  CUtensorMap ma, mw;
+  if (!make_map(&mw, w, w_rows, k, ldw, 128) || !make_map(&ma, a, p.m, k, lda, BN)) TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: cannot describe the operands to the copy unit");
+  const int tiles = (p.n + 127) / 128, row_tiles = (p.m + BN - 1) / BN;
+  // as many slices as two CTAs per SM take (148 SMs), eight at most, two groups at least in each
+  FewArgs f;
+  f.slices = max(1, min(min(8, p.groups / 2), 296 / (tiles * row_tiles)));
+  f.per_slice = (p.groups + f.slices - 1) / f.slices;
+  f.slices = (p.groups + f.per_slice - 1) / f.per_slice;
+  TLLM_REQUIRE(tiles <= 65535, "linear_fp8: %d columns are too many for one launch", p.n);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(row_tiles, tiles, f.slices);
+  cfg.blockDim = dim3(GATED ? 320 : 192);
+  cfg.dynamicSmemBytes = L::TOTAL;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = f.slices;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mw, ma, p, f, status);
+  if (e != cudaSuccess) TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: %s", cudaGetErrorString(e));
+  return TLLM_OK;
+}
+
 }  // namespace tllm
 
 using namespace tllm;
@@ -355,6 +629,20 @@ extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
   p.vec_out = (uintptr_t)out % 16 == 0 && (ldo * size) % 16 == 0;
   TLLM_REQUIRE(mode != OUT_FP8 || p.vec_out, "linear_fp8: rows of 8-bit values start on 16 bytes");
   cudaStream_t s = (cudaStream_t)stream;
-  if (gated) return launch_tiles<256, 4, true>(p, a, lda, w, ldw, 256 * ((n + 127) / 128), k, status, s);
-  return launch_tiles<128, 6, false>(p, a, lda, w, ldw, n, k, status, s);
+  const int w_rows = gated ? 256 * ((n + 127) / 128) : n;
+#define TLLM_FEW(BN, STAGES, GATED) return launch_few<BN, STAGES, GATED>(p, a, lda, w, ldw, w_rows, k, status, s)
+  if (m <= 128) {
+    if (gated) {
+      if (m <= 16) TLLM_FEW(16, 3, true);
+      if (m <= 32) TLLM_FEW(32, 3, true);
+      TLLM_FEW(64, 5, true);
+    }
+    if (m <= 16) TLLM_FEW(16, 6, false);
+    if (m <= 32) TLLM_FEW(32, 5, false);
+    if (m <= 64) TLLM_FEW(64, 4, false);
+    TLLM_FEW(128, 3, false);
+  }
+#undef TLLM_FEW
+  if (gated) return launch_tiles<256, 4, true>(p, a, lda, w, ldw, w_rows, k, status, s);
+  return launch_tiles<128, 6, false>(p, a, lda, w, ldw, w_rows, k, status, s);
 }
