@@ -12,6 +12,7 @@
 //
 // Sizes: any M, N and K; rows of A and W start on 16 bytes.  TMA fills the tails with zeros, the epilogue masks them.  Every wait
 // is bounded: on expiry the kernel records a code in `status`, stops issuing, frees its tensor memory and returns.
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -27,11 +28,28 @@ constexpr int BM = 128;          // rows of A per CTA = MMA M
 constexpr int BK = FP8_GROUP;    // values of K per stage: one group, one 128-byte swizzle row
 constexpr int UMMA_K = 32;
 constexpr int SUM_WARPS = 8;     // warps that scale and add: two per 32 rows, half of the columns each
-constexpr int THREADS = 64 + 32 * SUM_WARPS;   // warp 0: TMA, warp 1: MMA + tensor-memory allocation
+constexpr int FIRST_SUM_WARP = 4;  // warp 0: TMA, warp 1: MMA + tensor-memory allocation, 2 and 3 fill the warpgroup
+constexpr int THREADS = 32 * (FIRST_SUM_WARP + SUM_WARPS);
+// Registers: the launch gives 168 to each of 384 threads; the first warpgroup hands most of its own to the two that sum
+// (128 * 40 + 256 * 232 = 384 * 168).
+constexpr int REGS_OTHERS = 40, REGS_SUMS = 232;
+
+constexpr int BAND = 12;         // row tiles per band of the large products' order
 
 enum Output { OUT_BF16 = 0, OUT_F32 = 1, OUT_ADD = 2, OUT_FP8 = 3 };
 enum Act { ACT_SILU = 0, ACT_RELU = 1, ACT_CLAMPED = 2, ACT_GELU_TANH = 3 };
 
+// act(g) * u for all four gates without a branch (the code is laid out 64 times per thread): with g and u clamped,
+// g / (1 + exp(-g (a + b g^2))) * (c u + d).  SiLU: a = 1; GELU's tanh form z / 2 (1 + tanh(y)) = z / (1 + exp(-2 y)): a = 2 sqrt(2 / pi),
+// b = 0.044715 a; clamped: a = 1.702, d = 1; ReLU: g from 0 on, a = 0, so that 1 / (1 + 1) meets c = 2.
+struct Gate { float g_low, g_high, u_most, a, b, c, d; };
+static Gate make_gate(int act, float limit) {
+  const float inf = INFINITY;
+  if (act == ACT_RELU) return {0.f, inf, inf, 0.f, 0.f, 2.f, 0.f};
+  if (act == ACT_CLAMPED) return {-inf, limit, limit, 1.702f, 0.f, 1.f, 1.f};
+  if (act == ACT_GELU_TANH) return {-inf, inf, inf, 1.59576912160573081f, 1.59576912160573081f * 0.044715f, 1.f, 0.f};
+  return {-inf, inf, inf, 1.f, 0.f, 1.f, 0.f};
+}
 struct Fp8Args {
   const uint8_t* a_scales;     // [m][lda_s] e8m0
   const float* w_scales;       // [ceil(n / 128)][groups]
@@ -39,20 +57,19 @@ struct Fp8Args {
   uint8_t* out_scales;         // OUT_FP8: [m][ldo_s] e8m0
   long long lda_s, ldo, ldo_s;
   int m, n, groups;            // n: columns of `out` (gated: half the weight's rows, without the ones that fill the last block)
-  int mode, act;
-  float limit;
+  int mode;
   int vec_out;                 // rows of `out` start on 16 bytes
+  int vec_scales;              // rows of a_scales start on 4 bytes
+  Gate gate;
 };
 
-__device__ __forceinline__ float gate_f(float g, float u, int act, float limit) {
-  if (act == ACT_SILU) return g / (1.f + expf(-g)) * u;
-  if (act == ACT_RELU) return fmaxf(g, 0.f) * u;
-  if (act == ACT_CLAMPED) {
-    g = fminf(g, limit);
-    u = fminf(fmaxf(u, -limit), limit);
-    return g / (1.f + expf(-1.702f * g)) * (u + 1.f);
-  }
-  return g / (1.f + expf(-1.59576912160573081f * g * fmaf(0.044715f * g, g, 1.f))) * u;   // 2 sqrt(2 / pi)
+// (a NaN stays one)
+__device__ __forceinline__ float max_nan(float x, float y) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ float min_nan(float x, float y) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ float gate_f(float g, float u, const Gate& q) {
+  g = min_nan(max_nan(g, q.g_low), q.g_high);
+  u = min_nan(max_nan(u, -q.u_most), q.u_most);
+  return __fdividef(g, 1.f + expf(-g * fmaf(q.b * g, g, q.a))) * fmaf(q.c, u, q.d);
 }
 
 // e4m3 x e4m3 -> float32, M = m, N = n, both operands K-major (bits 7-9 and 10-12: 0 is e4m3)
@@ -65,6 +82,16 @@ __device__ __forceinline__ void umma_fp8_lo(uint32_t d_tmem, uint32_t a_lo, uint
       "mov.b64 db, {%2, %5};\n\t"
       "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n\t}"
       ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(SMEM_DESC_SW128_HI) : "memory");
+}
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+// Waits for this warp's loads from tensor memory; naming the registers keeps the arithmetic on them behind the wait.
+__device__ __forceinline__ void tmem_ld32_arrived(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                 "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                 "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
 // true in all the summing warps only if `ok` holds in all of them
 __device__ __forceinline__ bool sums_all(bool ok) {
@@ -176,82 +203,116 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   pdl_trigger();
   pdl_wait();
 
-  if (warp == 0) {
-    if (lane == 0) {
+  // Tile t: the row tiles in bands of BAND, inside a band the row tiles of one column of tiles are neighbours.  The tiles that run side
+  // by side then share both operands: about 12 x 12 of them instead of all row tiles by two or three columns.
+  auto tile_at = [&](int t, int& tm, int& tn) {
+    const int band = t / (BAND * tiles_n), first = band * BAND, high = min(BAND, tiles_m - first), in = t - band * BAND * tiles_n;
+    tm = first + in % high;
+    tn = in / high;
+  };
+
+  if (warp < FIRST_SUM_WARP) {
+    regs_down<REGS_OTHERS>();
+    if (warp == 0 && lane == 0) {
       // ---------------- TMA producer
       int it = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x)
+      for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x) {
+        int tm, tn;
+        tile_at(t, tm, tn);
         for (int g = 0; g < p.groups; ++g, ++it) {
           const int s = it % STAGES;
           if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { *abort_flag = 1; atomicExch(status, ERR_F8_PRODUCER); ok = false; break; }
           uint8_t* dst = smem + s * L::STAGE_BYTES;
           mbar_expect_tx(&full_bar[s], L::STAGE_BYTES);
-          tma_load_2d(dst, &map_a, g * BK, (t % tiles_m) * BM, &full_bar[s]);
-          tma_load_2d(dst + L::A_BYTES, &map_w, g * BK, (t / tiles_m) * BN, &full_bar[s]);
+          tma_load_2d(dst, &map_a, g * BK, tm * BM, &full_bar[s]);
+          tma_load_2d(dst + L::A_BYTES, &map_w, g * BK, tn * BN, &full_bar[s]);
         }
-      mbar_drain(full_bar, STAGES, it);
-    }
-  } else if (warp == 1) {
-    // ---------------- MMA issuer (warp-wide loop, one elected lane issues)
-    const uint32_t idesc = instr_desc_e4m3(BM, BN);
-    const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
-    const uint32_t lo0 = smem_desc_sw128_lo(smem_u32(smem));
-    int it = 0;
-    bool ok = true;
-    for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x)
-      for (int g = 0; g < p.groups; ++g, ++it) {
-        const int s = it % STAGES, buf = it & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, abort_flag) && mbar_wait(&full_bar[s], (it / STAGES) & 1, abort_flag));
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t a_lo = lo0 + s * (L::STAGE_BYTES >> 4), b_lo = a_lo + (L::A_BYTES >> 4);
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < BK / UMMA_K; ++k)
-            umma_fp8_lo(tmem_u + buf * BN, a_lo + (k * UMMA_K >> 4), b_lo + (k * UMMA_K >> 4), idesc, k > 0 ? 1u : 0u);
-          umma_commit(&empty_bar[s]);
-          umma_commit(&acc_full[buf]);
-        }
-        __syncwarp();
       }
-    if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_MMA); }
+      mbar_drain(full_bar, STAGES, it);
+    } else if (warp == 1) {
+      // ---------------- MMA issuer (warp-wide loop, one elected lane issues)
+      const uint32_t idesc = instr_desc_e4m3(BM, BN);
+      const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
+      const uint32_t lo0 = smem_desc_sw128_lo(smem_u32(smem));
+      int it = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x)
+        for (int g = 0; g < p.groups; ++g, ++it) {
+          const int s = it % STAGES, buf = it & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, abort_flag) && mbar_wait(&full_bar[s], (it / STAGES) & 1, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a_lo = lo0 + s * (L::STAGE_BYTES >> 4), b_lo = a_lo + (L::A_BYTES >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < BK / UMMA_K; ++k)
+              umma_fp8_lo(tmem_u + buf * BN, a_lo + (k * UMMA_K >> 4), b_lo + (k * UMMA_K >> 4), idesc, k > 0 ? 1u : 0u);
+            umma_commit(&empty_bar[s]);
+            umma_commit(&acc_full[buf]);
+          }
+          __syncwarp();
+        }
+      if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_MMA); }
+    }
   } else {
+    regs_up<REGS_SUMS>();
     // ---------------- sums: warp w reads tensor-memory lanes [32 (w % 4), +32), and of its row half the columns: with a plain
     // tile [half * BN / 2, +BN / 2), with a gated one 64 gate columns and the 64 matching up columns
     constexpr int COLS = BN / 2, CHUNKS = COLS / 32;
-    const int quad = warp & 3, half = (warp - 2) >> 2;
+    const int quad = warp & 3, half = (warp - FIRST_SUM_WARP) >> 2;
     const int row = quad * 32 + lane;
     auto column = [&](int c) { return GATED ? (c < CHUNKS / 2 ? half * 64 + 32 * c : 128 + half * 64 + 32 * (c - CHUNKS / 2)) : half * COLS + 32 * c; };
     int it = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < n_tiles; t += gridDim.x) {
-      const int m = (t % tiles_m) * BM + row, tile_n = t / tiles_m;
+      int tm, tile_n;
+      tile_at(t, tm, tile_n);
+      const int m = tm * BM + row;
+      // the row's scales, four groups to a word where the rows allow it
       const uint8_t* sa = p.a_scales + (long long)min(m, p.m - 1) * p.lda_s;
+      auto four_scales = [&](int g) -> uint32_t {
+        if (g >= p.groups) return 0u;
+        if (p.vec_scales && g + 4 <= p.groups) return *reinterpret_cast<const uint32_t*>(sa + g);
+        uint32_t q = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (g + e < p.groups) q |= (uint32_t)sa[g + e] << (8 * e);
+        return q;
+      };
       // the rows of W that a thread reads lie in one block of 128 (gated: one of gate, one of up), the last one where W ends inside a tile
       const int block = GATED ? 2 * tile_n : min((tile_n * BN + half * COLS) / 128, (p.n - 1) / 128);
       const float* sw = p.w_scales + (long long)block * p.groups;
       float acc[COLS];
 #pragma unroll
       for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
+      uint32_t quad_now = 0u, quad_next = four_scales(0);
+      float w0 = sw[0], w1 = GATED ? sw[p.groups] : 0.f;
       for (int g = 0; g < p.groups; ++g, ++it) {
         const int buf = it & 1;
-        const float a = fp8_scale(sa[g]), s0 = a * sw[g], s1 = GATED ? a * sw[p.groups + g] : s0;
+        if ((g & 3) == 0) { quad_now = quad_next; quad_next = four_scales(g + 4); }
+        const float a = fp8_scale((quad_now >> (8 * (g & 3))) & 255u), s0 = a * w0, s1 = a * w1;
+        if (g + 1 < p.groups) { w0 = sw[g + 1]; if (GATED) w1 = sw[p.groups + g + 1]; }
         ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (it >> 1) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
         const uint32_t taddr = tmem_base + buf * BN + ((uint32_t)(quad * 32) << 16);
+        uint32_t v[2][32];       // the next 32 columns are on their way while these are added
+        tmem_ld32_issue(taddr + column(0), v[0]);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-          float v[32];
-          tmem_ld32(taddr + column(c), v);
+          tmem_ld32_arrived(v[c & 1]);
+          if (c + 1 < CHUNKS) {
+            tmem_ld32_issue(taddr + column(c + 1), v[(c + 1) & 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[buf]);
+          }
           const float s = GATED && c >= CHUNKS / 2 ? s1 : s0;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) acc[32 * c + j] = fmaf(v[j], s, acc[32 * c + j]);
+          for (int j = 0; j < 32; ++j) acc[32 * c + j] = fmaf(__uint_as_float(v[c & 1][j]), s, acc[32 * c + j]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[buf]);
       }
       if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_SUMS); }
       if (!sums_all(ok)) break;
@@ -261,7 +322,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       } else {
         const int n = tile_n * 128 + half * 64;
 #pragma unroll
-        for (int j = 0; j < 64; ++j) acc[j] = n + j < p.n ? gate_f(acc[j], acc[64 + j], p.act, p.limit) : 0.f;
+        for (int j = 0; j < 64; ++j) acc[j] = n + j < p.n ? gate_f(acc[j], acc[64 + j], p.gate) : 0.f;
         if (p.mode != OUT_FP8) {
           store_columns<32>(p, m, n, acc, OUT_BF16);
           store_columns<32>(p, m, n + 32, acc + 32, OUT_BF16);
@@ -487,7 +548,7 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     }
     if (GATED) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[0][e] = n + e < p.n ? gate_f(sum[0][e], sum[TILES - 1][e], p.act, p.limit) : 0.f;
+      for (int e = 0; e < 4; ++e) sum[0][e] = n + e < p.n ? gate_f(sum[0][e], sum[TILES - 1][e], p.gate) : 0.f;
     }
     if (GATED && p.mode == OUT_FP8) {
       const uint32_t byte = fp8_scale_byte(__reduce_max_sync(0xffffffffu, max(max(fp8_abs_bits(sum[0][0]), fp8_abs_bits(sum[0][1])),
@@ -563,6 +624,14 @@ static int launch_tiles(const Fp8Args& p, const void* a, long long lda, const vo
   TLLM_RESERVE_SMEM("linear_fp8", L::TOTAL, kern);
   CUtensorMap ma, mw;
   if (!make_map(&ma, a, p.m, k, lda, BM) || !make_map(&mw, w, w_rows, k, ldw, BN)) TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: cannot describe the operands to the copy unit");
+  // the registers that the summing warpgroups ask for are those of the launch, or they would wait for good
+  static int regs = 0;
+  if (regs == 0) {
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess) TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: cannot read the kernel's registers");
+    regs = fa.numRegs;
+  }
+  TLLM_REQUIRE(regs * THREADS >= 128 * REGS_OTHERS + 32 * SUM_WARPS * REGS_SUMS, "linear_fp8: built with %d registers, too few for its split", regs);
   const int tiles = ((p.m + BM - 1) / BM) * (GATED ? (p.n + 127) / 128 : (p.n + BN - 1) / BN);
   int dev = 0, sm_count = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sm_count < 1)
@@ -624,9 +693,10 @@ extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
   p.a_scales = (const uint8_t*)a_scales; p.w_scales = w_scales; p.out = out; p.out_scales = (uint8_t*)out_scales;
   p.lda_s = lda_s; p.ldo = ldo; p.ldo_s = ldo_s;
   p.m = m; p.n = n; p.groups = (k + BK - 1) / BK;
-  p.mode = mode; p.act = act; p.limit = limit;
+  p.mode = mode; p.gate = make_gate(act, limit);
   const int size = mode == OUT_BF16 ? 2 : (mode == OUT_FP8 ? 1 : 4);
   p.vec_out = (uintptr_t)out % 16 == 0 && (ldo * size) % 16 == 0;
+  p.vec_scales = (uintptr_t)a_scales % 4 == 0 && lda_s % 4 == 0;
   TLLM_REQUIRE(mode != OUT_FP8 || p.vec_out, "linear_fp8: rows of 8-bit values start on 16 bytes");
   cudaStream_t s = (cudaStream_t)stream;
   const int w_rows = gated ? 256 * ((n + 127) / 128) : n;
@@ -644,5 +714,6 @@ extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
   }
 #undef TLLM_FEW
   if (gated) return launch_tiles<256, 4, true>(p, a, lda, w, ldw, w_rows, k, status, s);
+  if (p.n > 128 && (long long)((m + 127) / 128) * ((n + 255) / 256) >= 74) return launch_tiles<256, 4, false>(p, a, lda, w, ldw, w_rows, k, status, s);
   return launch_tiles<128, 6, false>(p, a, lda, w, ldw, w_rows, k, status, s);
 }

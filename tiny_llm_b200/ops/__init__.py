@@ -1502,10 +1502,10 @@ def _fp8_groups(k: int) -> int:
 
 
 def fp8_rows(m: int, k: int, device):
-    """Room for 8-bit rows: (values e4m3 [m, k], whose rows start on 16 bytes, and scales e8m0 [m, ceil(k / 128)]).  The
-    values are a view where k is no multiple of 16; what lies behind a row's end is never read or written."""
+    """Room for 8-bit rows: (values e4m3 [m, k], whose rows start on 16 bytes, and scales e8m0 [m, ceil(k / 128)],
+    whose rows do so too).  Both may be views of wider rows; what lies behind a row's end is never read or written."""
     data = torch.empty(m, -(-k // 16) * 16, dtype=FP8, device=device)[:, :k]
-    return data, torch.empty(m, _fp8_groups(k), dtype=FP8_SCALE, device=device)
+    return data, torch.empty(m, -(-_fp8_groups(k) // 16) * 16, dtype=FP8_SCALE, device=device)[:, : _fp8_groups(k)]
 
 
 def fp8_weight(n: int, k: int, device):
