@@ -27,13 +27,12 @@ namespace tllm {
 constexpr int BM = 128;          // rows of A per CTA = MMA M
 constexpr int BK = FP8_GROUP;    // values of K per stage: one group, one 128-byte swizzle row
 constexpr int UMMA_K = 32;
-constexpr int SUM_WARPS = 8;     // warps that scale and add: two per 32 rows, half of the columns each
+constexpr int SUM_WARPS = 16;    // warps that scale and add: four per 32 rows, a quarter of the columns each
 constexpr int FIRST_SUM_WARP = 4;  // warp 0: TMA, warp 1: MMA + tensor-memory allocation, 2 and 3 fill the warpgroup
 constexpr int THREADS = 32 * (FIRST_SUM_WARP + SUM_WARPS);
-// Registers: the launch gives 168 to each of 384 threads; the first warpgroup hands most of its own to the two that sum
-// (128 * 40 + 256 * 232 = 384 * 168).
-constexpr int REGS_OTHERS = 40, REGS_SUMS = 232;
-
+// Registers: the launch gives 96 to each of 640 threads; the first warpgroup hands most of its own to the four that sum
+// (128 * 32 + 512 * 112 = 640 * 96).
+constexpr int REGS_OTHERS = 32, REGS_SUMS = 112;
 constexpr int BAND = 12;         // row tiles per band of the large products' order
 
 enum Output { OUT_BF16 = 0, OUT_F32 = 1, OUT_ADD = 2, OUT_FP8 = 3 };
@@ -93,6 +92,16 @@ __device__ __forceinline__ void tmem_ld32_arrived(uint32_t* r) {
                  "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
                  "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
+// (c0, c1) + (a0, a1) * s in one instruction
+__device__ __forceinline__ float2 fma2(uint32_t a0, uint32_t a1, float2 s, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "r"(a0), "r"(a1), "f"(s.x), "f"(s.y), "f"(c.x), "f"(c.y));
+  return r;
+}
 // true in all the summing warps only if `ok` holds in all of them
 __device__ __forceinline__ bool sums_all(bool ok) {
   uint32_t r;
@@ -120,8 +129,8 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr, uint32_t rank)
 template <int BN, int STAGES>
 struct Smem {
   static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK, STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int MOST_OFFSET = STAGES * STAGE_BYTES;           // the largest magnitudes of a row's two halves
-  static constexpr int BAR_OFFSET = MOST_OFFSET + 2 * BM * 4;
+  static constexpr int MOST_OFFSET = STAGES * STAGE_BYTES;           // the largest magnitudes of a row's four parts
+  static constexpr int BAR_OFFSET = MOST_OFFSET + 4 * BM * 4;
   static constexpr int TOTAL = BAR_OFFSET + (2 * STAGES + 4) * 8 + 16 + 1024;
 };
 
@@ -257,12 +266,12 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     }
   } else {
     regs_up<REGS_SUMS>();
-    // ---------------- sums: warp w reads tensor-memory lanes [32 (w % 4), +32), and of its row half the columns: with a plain
-    // tile [half * BN / 2, +BN / 2), with a gated one 64 gate columns and the 64 matching up columns
-    constexpr int COLS = BN / 2, CHUNKS = COLS / 32;
-    const int quad = warp & 3, half = (warp - FIRST_SUM_WARP) >> 2;
+    // ---------------- sums: warp w reads tensor-memory lanes [32 (w % 4), +32), and of its row a quarter of the columns: with a
+    // plain tile [part * BN / 4, +BN / 4), with a gated one 32 gate columns and the 32 matching up columns
+    constexpr int COLS = BN / 4, CHUNKS = COLS / 32;
+    const int quad = warp & 3, part = (warp - FIRST_SUM_WARP) >> 2;
     const int row = quad * 32 + lane;
-    auto column = [&](int c) { return GATED ? (c < CHUNKS / 2 ? half * 64 + 32 * c : 128 + half * 64 + 32 * (c - CHUNKS / 2)) : half * COLS + 32 * c; };
+    auto column = [&](int c) { return GATED ? part * 32 + 128 * c : part * COLS + 32 * c; };
     int it = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < n_tiles; t += gridDim.x) {
@@ -281,7 +290,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         return q;
       };
       // the rows of W that a thread reads lie in one block of 128 (gated: one of gate, one of up), the last one where W ends inside a tile
-      const int block = GATED ? 2 * tile_n : min((tile_n * BN + half * COLS) / 128, (p.n - 1) / 128);
+      const int block = GATED ? 2 * tile_n : min((tile_n * BN + part * COLS) / 128, (p.n - 1) / 128);
       const float* sw = p.w_scales + (long long)block * p.groups;
       float acc[COLS];
 #pragma unroll
@@ -297,21 +306,23 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         if (!ok) break;
         tc_fence_after();
         const uint32_t taddr = tmem_base + buf * BN + ((uint32_t)(quad * 32) << 16);
-        uint32_t v[2][32];       // the next 32 columns are on their way while these are added
-        tmem_ld32_issue(taddr + column(0), v[0]);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-          tmem_ld32_arrived(v[c & 1]);
-          if (c + 1 < CHUNKS) {
-            tmem_ld32_issue(taddr + column(c + 1), v[(c + 1) & 1]);
-          } else {
+          uint32_t v[32];
+          tmem_ld32_issue(taddr + column(c), v);
+          tmem_ld32_arrived(v);
+          if (c == CHUNKS - 1) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&acc_empty[buf]);
           }
-          const float s = GATED && c >= CHUNKS / 2 ? s1 : s0;
+          const float s = GATED && c > 0 ? s1 : s0;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) acc[32 * c + j] = fmaf(__uint_as_float(v[c & 1][j]), s, acc[32 * c + j]);
+          for (int j = 0; j < 32; j += 2) {
+            const float2 r = fma2(v[j], v[j + 1], make_float2(s, s), make_float2(acc[32 * c + j], acc[32 * c + j + 1]));
+            acc[32 * c + j] = r.x;
+            acc[32 * c + j + 1] = r.y;
+          }
         }
       }
       if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_SUMS); }
@@ -320,25 +331,24 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) store_columns<32>(p, m, tile_n * BN + column(c), acc + 32 * c, p.mode);
       } else {
-        const int n = tile_n * 128 + half * 64;
+        const int n = tile_n * 128 + part * 32;
 #pragma unroll
-        for (int j = 0; j < 64; ++j) acc[j] = n + j < p.n ? gate_f(acc[j], acc[64 + j], p.gate) : 0.f;
+        for (int j = 0; j < 32; ++j) acc[j] = n + j < p.n ? gate_f(acc[j], acc[32 + j], p.gate) : 0.f;
         if (p.mode != OUT_FP8) {
           store_columns<32>(p, m, n, acc, OUT_BF16);
-          store_columns<32>(p, m, n + 32, acc + 32, OUT_BF16);
         } else {
           uint32_t largest = 0u;
 #pragma unroll
-          for (int j = 0; j < 64; ++j) largest = max(largest, fp8_abs_bits(acc[j]));
-          most[half * BM + row] = largest;
+          for (int j = 0; j < 32; ++j) largest = max(largest, fp8_abs_bits(acc[j]));
+          most[part * BM + row] = largest;
           sums_all(true);
-          const uint32_t byte = fp8_scale_byte(max(most[row], most[BM + row]));
+          const uint32_t byte = fp8_scale_byte(max(max(most[row], most[BM + row]), max(most[2 * BM + row], most[3 * BM + row])));
           const float inverse = fp8_inverse_scale(byte);
           if (m < p.m) {
             uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + (size_t)m * p.ldo + n;
-            if (half == 0) p.out_scales[(size_t)m * p.ldo_s + tile_n] = (uint8_t)byte;
+            if (part == 0) p.out_scales[(size_t)m * p.ldo_s + tile_n] = (uint8_t)byte;
 #pragma unroll
-            for (int j = 0; j < 64; j += 16) {
+            for (int j = 0; j < 32; j += 16) {
               uint4 pk;
               pk.x = fp8_pack4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3], inverse, byte);
               pk.y = fp8_pack4(acc[j + 4], acc[j + 5], acc[j + 6], acc[j + 7], inverse, byte);
@@ -631,7 +641,7 @@ static int launch_tiles(const Fp8Args& p, const void* a, long long lda, const vo
     if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess) TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: cannot read the kernel's registers");
     regs = fa.numRegs;
   }
-  TLLM_REQUIRE(regs * THREADS >= 128 * REGS_OTHERS + 32 * SUM_WARPS * REGS_SUMS, "linear_fp8: built with %d registers, too few for its split", regs);
+  TLLM_REQUIRE(regs * THREADS >= 32 * FIRST_SUM_WARP * REGS_OTHERS + 32 * SUM_WARPS * REGS_SUMS, "linear_fp8: built with %d registers, too few for its split", regs);
   const int tiles = ((p.m + BM - 1) / BM) * (GATED ? (p.n + 127) / 128 : (p.n + BN - 1) / BN);
   int dev = 0, sm_count = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sm_count < 1)
