@@ -131,7 +131,8 @@ struct Smem {
   static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK, STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int MOST_OFFSET = STAGES * STAGE_BYTES;           // the largest magnitudes of a row's four parts
   static constexpr int BAR_OFFSET = MOST_OFFSET + 4 * BM * 4;
-  static constexpr int TOTAL = BAR_OFFSET + (2 * STAGES + 4) * 8 + 16 + 1024;
+  static constexpr int ACCS = 512 / BN;            // accumulators in tensor memory: the products run that many groups ahead of the sums
+  static constexpr int TOTAL = BAR_OFFSET + (2 * STAGES + 2 * ACCS) * 8 + 16 + 1024;
 };
 
 // eight columns as bfloat16
@@ -183,14 +184,15 @@ __global__ void __launch_bounds__(THREADS, 1)
 linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const Fp8Args p, int* __restrict__ status) {
   static_assert(!GATED || BN == 256, "a gated tile is one group of gate columns and one of up columns");
   using L = Smem<BN, STAGES>;
+  constexpr int ACCS = L::ACCS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint32_t* most = reinterpret_cast<uint32_t*>(smem + L::MOST_OFFSET);
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::BAR_OFFSET);
   uint64_t* empty_bar = full_bar + STAGES;
-  uint64_t* acc_full = empty_bar + STAGES;      // [2]: accumulator b holds a group's products
-  uint64_t* acc_empty = acc_full + 2;           // [2]: the summing warps have read accumulator b
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* acc_full = empty_bar + STAGES;      // accumulator b holds a group's products
+  uint64_t* acc_empty = acc_full + ACCS;        // the summing warps have read accumulator b
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + ACCS);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -200,11 +202,11 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   if (threadIdx.x == 0) {
     tma_prefetch_map(&map_a); tma_prefetch_map(&map_w);
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], SUM_WARPS); }
+    for (int b = 0; b < ACCS; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], SUM_WARPS); }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) tmem_alloc(tmem_slot, 2 * BN);
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -248,8 +250,8 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       bool ok = true;
       for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x)
         for (int g = 0; g < p.groups; ++g, ++it) {
-          const int s = it % STAGES, buf = it & 1;
-          ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, abort_flag) && mbar_wait(&full_bar[s], (it / STAGES) & 1, abort_flag));
+          const int s = it % STAGES, buf = it % ACCS;
+          ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((it / ACCS) & 1) ^ 1, abort_flag) && mbar_wait(&full_bar[s], (it / STAGES) & 1, abort_flag));
           if (!ok) break;
           tc_fence_after();
           const uint32_t a_lo = lo0 + s * (L::STAGE_BYTES >> 4), b_lo = a_lo + (L::A_BYTES >> 4);
@@ -298,11 +300,11 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       uint32_t quad_now = 0u, quad_next = four_scales(0);
       float w0 = sw[0], w1 = GATED ? sw[p.groups] : 0.f;
       for (int g = 0; g < p.groups; ++g, ++it) {
-        const int buf = it & 1;
+        const int buf = it % ACCS;
         if ((g & 3) == 0) { quad_now = quad_next; quad_next = four_scales(g + 4); }
         const float a = fp8_scale((quad_now >> (8 * (g & 3))) & 255u), s0 = a * w0, s1 = a * w1;
         if (g + 1 < p.groups) { w0 = sw[g + 1]; if (GATED) w1 = sw[p.groups + g + 1]; }
-        ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (it >> 1) & 1, abort_flag));
+        ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (it / ACCS) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
         const uint32_t taddr = tmem_base + buf * BN + ((uint32_t)(quad * 32) << 16);
@@ -370,7 +372,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem_base, 2 * BN);
+  if (warp == 1) tmem_dealloc(tmem_base, 512);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -380,14 +382,17 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 // CTAs share the tile's tokens, a warp per token: it adds the slices over the peers' shared memory in a fixed order, four weight rows
 // per lane, and stores 128 neighbouring columns.  Gated: a CTA has the gate tile and the up tile beside it, two accumulators and four
 // warps for each; the 128 columns that a warp stores are one group of the product behind.
-constexpr int FEW_CHUNK = 16;    // groups whose scales (of the row times of the block) are laid out in shared memory at a time
+// A tile's columns are dealt to HALVES sets of four summing warps.
+constexpr int FEW_CHUNK = 8;     // groups whose scales (of the row times of the block) are laid out in shared memory at a time
 
-template <int BN, int STAGES, bool GATED>
+template <int BN, int STAGES, bool GATED, int HALVES>
 struct FewSmem {
+  static constexpr int SUM_WARPS = 4 * (GATED ? 2 : 1) * HALVES, THREADS = 64 + 32 * SUM_WARPS;
   static constexpr int TILES = GATED ? 2 : 1, W_BYTES = TILES * 128 * BK, A_BYTES = BN * BK, STAGE_BYTES = W_BYTES + A_BYTES;
   static constexpr int SCALE_OFFSET = STAGES * STAGE_BYTES;
   static constexpr int BAR_OFFSET = SCALE_OFFSET + TILES * FEW_CHUNK * BN * 4;
   static constexpr int TOTAL = BAR_OFFSET + (2 * STAGES + 4) * 8 + 16 + 1024;
+  static constexpr int RESIDENT = TOTAL <= 113 * 1024 && THREADS <= 320 ? 2 : 1;     // CTAs per SM
   static_assert(TILES * BN * 128 * 4 <= STAGES * STAGE_BYTES, "the sums are left where the stages were");
 };
 
@@ -395,11 +400,11 @@ struct FewArgs {
   int slices, per_slice;       // slices of K (the cluster), groups per slice (the last may have fewer, or none)
 };
 
-template <int BN, int STAGES, bool GATED>
-__global__ void __launch_bounds__(GATED ? 320 : 192, (FewSmem<BN, STAGES, GATED>::TOTAL <= 113 * 1024) ? 2 : 1)
+template <int BN, int STAGES, bool GATED, int HALVES>
+__global__ void __launch_bounds__(FewSmem<BN, STAGES, GATED, HALVES>::THREADS, FewSmem<BN, STAGES, GATED, HALVES>::RESIDENT)
 linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const Fp8Args p, const FewArgs f, int* __restrict__ status) {
-  using L = FewSmem<BN, STAGES, GATED>;
-  constexpr int TILES = L::TILES, FEW_SUM_WARPS = 4 * TILES, WARPS = 2 + FEW_SUM_WARPS;
+  using L = FewSmem<BN, STAGES, GATED, HALVES>;
+  constexpr int TILES = L::TILES, FEW_SUM_WARPS = L::SUM_WARPS, WARPS = 2 + FEW_SUM_WARPS;
   constexpr uint32_t ACC_COLS = TILES * BN, TMEM_COLS = 2 * ACC_COLS < 32 ? 32 : 2 * ACC_COLS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -484,42 +489,66 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     }
     if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_MMA); }
   } else {
-    // ---------------- sums: warp w reads tensor-memory lanes [32 (w % 4), +32) of its tile's accumulator
-    const int quad = warp & 3, part = GATED ? (warp - 2) >> 2 : 0, thread = threadIdx.x - 64;
+    // ---------------- sums: warp w reads tensor-memory lanes [32 (w % 4), +32) of its tile's accumulator, COLS columns of it
+    constexpr int COLS = BN / HALVES;
+    const int quad = warp & 3, set = (warp - 2) >> 2, part = set / HALVES, col0 = (set % HALVES) * COLS, thread = threadIdx.x - 64;
     const int row = quad * 32 + lane;
-    float acc[BN];
+    float acc[COLS];
 #pragma unroll
-    for (int j = 0; j < BN; ++j) acc[j] = 0.f;
+    for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
+    // the scales of a chunk of groups: fetched while the chunk before is added up, the row's times the block's in shared memory
+    constexpr int FETCH = (FEW_CHUNK * BN + 32 * FEW_SUM_WARPS - 1) / (32 * FEW_SUM_WARPS);
+    float fetched[FETCH][TILES];
+    auto fetch = [&](int i0) {
+#pragma unroll
+      for (int q = 0; q < FETCH; ++q) {
+        const int e = thread + q * 32 * FEW_SUM_WARPS, g = e % FEW_CHUNK, j = e / FEW_CHUNK;
+        const bool there = j < BN && i0 + g < n_g && m0 + j < p.m;
+        const float a = there ? fp8_scale(p.a_scales[(long long)(m0 + j) * p.lda_s + g_begin + i0 + g]) : 0.f;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) fetched[q][t] = there ? a * p.w_scales[(long long)(tile * TILES + t) * p.groups + g_begin + i0 + g] : 0.f;
+      }
+    };
     bool ok = true;
+    fetch(0);
     for (int i0 = 0; i0 < n_g; i0 += FEW_CHUNK) {
       const int n = min(FEW_CHUNK, n_g - i0);
       asm volatile("bar.sync 1, %0;" ::"n"(32 * FEW_SUM_WARPS) : "memory");     // the chunk before has been read
-      for (int e = thread; e < FEW_CHUNK * BN; e += 32 * FEW_SUM_WARPS) {
-        const int g = e % FEW_CHUNK, j = e / FEW_CHUNK;
-        const float a = g < n && m0 + j < p.m ? fp8_scale(p.a_scales[(long long)(m0 + j) * p.lda_s + g_begin + i0 + g]) : 0.f;
+#pragma unroll
+      for (int q = 0; q < FETCH; ++q) {
+        const int e = thread + q * 32 * FEW_SUM_WARPS, g = e % FEW_CHUNK, j = e / FEW_CHUNK;
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
-          scale[(t * FEW_CHUNK + g) * BN + j] = g < n ? a * p.w_scales[(long long)(tile * TILES + t) * p.groups + g_begin + i0 + g] : 0.f;
+          if (j < BN) scale[(t * FEW_CHUNK + g) * BN + j] = fetched[q][t];
       }
       asm volatile("bar.sync 1, %0;" ::"n"(32 * FEW_SUM_WARPS) : "memory");
+      if (i0 + FEW_CHUNK < n_g) fetch(i0 + FEW_CHUNK);
       for (int g = 0; g < n && ok; ++g) {
         const int i = i0 + g, buf = i & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (i >> 1) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
-        const uint32_t taddr = tmem_base + buf * ACC_COLS + part * BN + ((uint32_t)(quad * 32) << 16);
-        const float4* sc = reinterpret_cast<const float4*>(scale + (part * FEW_CHUNK + g) * BN);
-#pragma unroll
-        for (int c = 0; c < BN; c += 16) {
+        const uint32_t taddr = tmem_base + buf * ACC_COLS + part * BN + col0 + ((uint32_t)(quad * 32) << 16);
+        const float4* sc = reinterpret_cast<const float4*>(scale + (part * FEW_CHUNK + g) * BN + col0);
+        auto add = [&](float* to, const uint32_t* v, int c) {      // four columns
+          const float4 s4 = sc[c / 4];
+          const float2 lo = fma2(v[0], v[1], make_float2(s4.x, s4.y), make_float2(to[0], to[1]));
+          const float2 hi = fma2(v[2], v[3], make_float2(s4.z, s4.w), make_float2(to[2], to[3]));
+          to[0] = lo.x; to[1] = lo.y; to[2] = hi.x; to[3] = hi.y;
+        };
+        if constexpr (COLS == 16) {
           float v[16];
-          tmem_ld16(taddr + c, v);
+          tmem_ld16(taddr, v);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 s4 = sc[c / 4 + j];
-            acc[c + 4 * j] = fmaf(v[4 * j], s4.x, acc[c + 4 * j]);
-            acc[c + 4 * j + 1] = fmaf(v[4 * j + 1], s4.y, acc[c + 4 * j + 1]);
-            acc[c + 4 * j + 2] = fmaf(v[4 * j + 2], s4.z, acc[c + 4 * j + 2]);
-            acc[c + 4 * j + 3] = fmaf(v[4 * j + 3], s4.w, acc[c + 4 * j + 3]);
+          for (int j = 0; j < 16; j += 4) add(acc + j, reinterpret_cast<const uint32_t*>(v) + j, j);
+        } else {
+#pragma unroll
+          for (int c = 0; c < COLS; c += 32) {
+            uint32_t v[32];
+            tmem_ld32_issue(taddr + c, v);
+            tmem_ld32_arrived(v);
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) add(acc + c + j, v + j, c + j);
           }
         }
         tc_fence_before();
@@ -529,9 +558,9 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     }
     if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_SUMS); }
     // the last accumulator is there, so every product has read its stage: the stages are free
-    float* mine = parked + part * BN * 128 + row;
+    float* mine = parked + (part * BN + col0) * 128 + row;
 #pragma unroll
-    for (int j = 0; j < BN; ++j) mine[j * 128] = acc[j];
+    for (int j = 0; j < COLS; ++j) mine[j * 128] = acc[j];
   }
   tc_fence_before();
   __syncthreads();
@@ -650,23 +679,23 @@ static int launch_tiles(const Fp8Args& p, const void* a, long long lda, const vo
   return TLLM_OK;
 }
 
-template <int BN, int STAGES, bool GATED>
+template <int BN, int STAGES, bool GATED, int HALVES>
 static int launch_few(const Fp8Args& p, const void* a, long long lda, const void* w, long long ldw, int w_rows, int k, int* status, cudaStream_t s) {
-  using L = FewSmem<BN, STAGES, GATED>;
-  auto kern = linear_fp8_few_kernel<BN, STAGES, GATED>;
+  using L = FewSmem<BN, STAGES, GATED, HALVES>;
+  auto kern = linear_fp8_few_kernel<BN, STAGES, GATED, HALVES>;
   TLLM_RESERVE_SMEM("linear_fp8", L::TOTAL, kern);
   CUtensorMap ma, mw;
   if (!make_map(&mw, w, w_rows, k, ldw, 128) || !make_map(&ma, a, p.m, k, lda, BN)) TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: cannot describe the operands to the copy unit");
   const int tiles = (p.n + 127) / 128, row_tiles = (p.m + BN - 1) / BN;
-  // as many slices as two CTAs per SM take (148 SMs), eight at most, two groups at least in each
+  // as many slices as the 148 SMs take, eight at most, four groups at least in each
   FewArgs f;
-  f.slices = max(1, min(min(8, p.groups / 2), 296 / (tiles * row_tiles)));
+  f.slices = max(1, min(min(8, p.groups / 4), 148 * L::RESIDENT / (tiles * row_tiles)));
   f.per_slice = (p.groups + f.slices - 1) / f.slices;
   f.slices = (p.groups + f.per_slice - 1) / f.per_slice;
   TLLM_REQUIRE(tiles <= 65535, "linear_fp8: %d columns are too many for one launch", p.n);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(row_tiles, tiles, f.slices);
-  cfg.blockDim = dim3(GATED ? 320 : 192);
+  cfg.blockDim = dim3(L::THREADS);
   cfg.dynamicSmemBytes = L::TOTAL;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -710,17 +739,17 @@ extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
   TLLM_REQUIRE(mode != OUT_FP8 || p.vec_out, "linear_fp8: rows of 8-bit values start on 16 bytes");
   cudaStream_t s = (cudaStream_t)stream;
   const int w_rows = gated ? 256 * ((n + 127) / 128) : n;
-#define TLLM_FEW(BN, STAGES, GATED) return launch_few<BN, STAGES, GATED>(p, a, lda, w, ldw, w_rows, k, status, s)
+#define TLLM_FEW(BN, STAGES, GATED, HALVES) return launch_few<BN, STAGES, GATED, HALVES>(p, a, lda, w, ldw, w_rows, k, status, s)
   if (m <= 128) {
     if (gated) {
-      if (m <= 16) TLLM_FEW(16, 3, true);
-      if (m <= 32) TLLM_FEW(32, 3, true);
-      TLLM_FEW(64, 5, true);
+      if (m <= 16) TLLM_FEW(16, 3, true, 1);
+      if (m <= 32) TLLM_FEW(32, 3, true, 1);
+      TLLM_FEW(64, 5, true, 2);
     }
-    if (m <= 16) TLLM_FEW(16, 6, false);
-    if (m <= 32) TLLM_FEW(32, 5, false);
-    if (m <= 64) TLLM_FEW(64, 4, false);
-    TLLM_FEW(128, 3, false);
+    if (m <= 16) TLLM_FEW(16, 6, false, 1);
+    if (m <= 32) TLLM_FEW(32, 5, false, 1);
+    if (m <= 64) TLLM_FEW(64, 4, false, 2);
+    TLLM_FEW(128, 6, false, 4);
   }
 #undef TLLM_FEW
   if (gated) return launch_tiles<256, 4, true>(p, a, lda, w, ldw, w_rows, k, status, s);
