@@ -33,7 +33,7 @@ constexpr int THREADS = 32 * (FIRST_SUM_WARP + SUM_WARPS);
 // Registers: the launch gives 96 to each of 640 threads; the first warpgroup hands most of its own to the four that sum
 // (128 * 32 + 512 * 112 = 640 * 96).
 constexpr int REGS_OTHERS = 32, REGS_SUMS = 112;
-constexpr int BAND_ROWS = 2048;  // rows per band of the large products' order
+constexpr int BAND = 12;         // row tiles per band of the large products' order
 
 enum Output { OUT_BF16 = 0, OUT_F32 = 1, OUT_ADD = 2, OUT_FP8 = 3 };
 enum Act { ACT_SILU = 0, ACT_RELU = 1, ACT_CLAMPED = 2, ACT_GELU_TANH = 3 };
@@ -117,43 +117,6 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// ---- a pair of CTAs on one tile (cta_group::2)
-__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {     // where `p` of this CTA lies in the CTA of that rank
-  uint32_t a;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  return a;
-}
-// (Nothing but reads of tensor memory, which have returned, comes before this arrival: it needs no release to the cluster, a fence that
-// took longer than all the rest of a group: 900 us instead of 400 for 8,192 rows of 4,096 x 14,336.)
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
-}
-// a copy into this CTA whose bytes are counted by a barrier of the pair's first CTA
-__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
-}
-__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst_smem, uint32_t cols) {
-  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)), "r"(cols) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
-  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
-}
-// arrives at the barrier in both CTAs of the pair when the products issued so far have completed
-__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
-}
-__device__ __forceinline__ void umma_fp8_pair_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "mov.b64 da, {%1, %5};\n\t"
-      "mov.b64 db, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %3, p;\n\t}"
-      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(SMEM_DESC_SW128_HI) : "memory");
-}
 // four floats at byte address `addr` of this CTA's shared memory, read from the CTA of rank `rank` in the cluster
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr, uint32_t rank) {
   uint32_t remote;
@@ -163,9 +126,9 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr, uint32_t rank)
   return v;
 }
 
-template <int BN, int STAGES, bool PAIR>
+template <int BN, int STAGES>
 struct Smem {
-  static constexpr int A_BYTES = BM * BK, B_BYTES = (PAIR ? BN / 2 : BN) * BK, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK, STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int MOST_OFFSET = STAGES * STAGE_BYTES;           // the largest magnitudes of a row's four parts
   static constexpr int BAR_OFFSET = MOST_OFFSET + 4 * BM * 4;
   static constexpr int ACCS = 512 / BN;            // accumulators in tensor memory: the products run that many groups ahead of the sums
@@ -216,15 +179,11 @@ __device__ __forceinline__ void store_columns(const Fp8Args& p, int m, int n, co
   }
 }
 
-// PAIR: two CTAs on neighbouring SMs share a tile of 256 x BN.  Each has 128 rows of A and half the rows of W in its shared memory, and
-// the sums of its own rows; one thread of the first CTA issues the products of both.  A CTA on its own fetches 48 KB for the 512 cycles
-// that the products of a 128 x 256 group take, and an SM gets no more than about 64 bytes a cycle from L2: 768 cycles.  In a pair it
-// fetches 32 KB.
-template <int BN, int STAGES, bool GATED, bool PAIR>
+template <int BN, int STAGES, bool GATED>
 __global__ void __launch_bounds__(THREADS, 1)
 linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const Fp8Args p, int* __restrict__ status) {
   static_assert(!GATED || BN == 256, "a gated tile is one group of gate columns and one of up columns");
-  using L = Smem<BN, STAGES, PAIR>;
+  using L = Smem<BN, STAGES>;
   constexpr int ACCS = L::ACCS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -237,32 +196,26 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int TILE_M = PAIR ? 2 * BM : BM, BAND = BAND_ROWS / TILE_M;
-  const int rank = PAIR ? blockIdx.x & 1 : 0, first_tile = PAIR ? blockIdx.x >> 1 : blockIdx.x, tile_step = PAIR ? gridDim.x >> 1 : gridDim.x;
-  const int tiles_m = (p.m + TILE_M - 1) / TILE_M, tiles_n = GATED ? (p.n + 127) / 128 : (p.n + BN - 1) / BN;
+  const int tiles_m = (p.m + BM - 1) / BM, tiles_n = GATED ? (p.n + 127) / 128 : (p.n + BN - 1) / BN;
   const int n_tiles = tiles_m * tiles_n;
 
   if (threadIdx.x == 0) {
     tma_prefetch_map(&map_a); tma_prefetch_map(&map_w);
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-    for (int b = 0; b < ACCS; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], PAIR ? 2 * SUM_WARPS : SUM_WARPS); }
+    for (int b = 0; b < ACCS; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], SUM_WARPS); }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) {
-    if (PAIR) tmem_alloc_pair(tmem_slot, 512);
-    else tmem_alloc(tmem_slot, 512);
-  }
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
-  if (PAIR) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_trigger();
   pdl_wait();
 
-  // Tile t: the row tiles in bands, inside a band the row tiles of one column of tiles are neighbours.  The tiles that run side by side
-  // then share both operands: a square of them instead of all row tiles by two or three columns.
+  // Tile t: the row tiles in bands of BAND, inside a band the row tiles of one column of tiles are neighbours.  The tiles that run side
+  // by side then share both operands: about 12 x 12 of them instead of all row tiles by two or three columns.
   auto tile_at = [&](int t, int& tm, int& tn) {
     const int band = t / (BAND * tiles_n), first = band * BAND, high = min(BAND, tiles_m - first), in = t - band * BAND * tiles_n;
     tm = first + in % high;
@@ -275,49 +228,39 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       // ---------------- TMA producer
       int it = 0;
       bool ok = true;
-      for (int t = first_tile; t < n_tiles && ok; t += tile_step) {
+      for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x) {
         int tm, tn;
         tile_at(t, tm, tn);
         for (int g = 0; g < p.groups; ++g, ++it) {
           const int s = it % STAGES;
           if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { *abort_flag = 1; atomicExch(status, ERR_F8_PRODUCER); ok = false; break; }
           uint8_t* dst = smem + s * L::STAGE_BYTES;
-          if (PAIR) {
-            const uint32_t bar = cluster_addr(&full_bar[s], 0);
-            if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * L::STAGE_BYTES);
-            tma_load_2d_pair(dst, &map_a, g * BK, tm * TILE_M + rank * BM, bar);
-            tma_load_2d_pair(dst + L::A_BYTES, &map_w, g * BK, tn * BN + rank * (BN / 2), bar);
-          } else {
-            mbar_expect_tx(&full_bar[s], L::STAGE_BYTES);
-            tma_load_2d(dst, &map_a, g * BK, tm * BM, &full_bar[s]);
-            tma_load_2d(dst + L::A_BYTES, &map_w, g * BK, tn * BN, &full_bar[s]);
-          }
+          mbar_expect_tx(&full_bar[s], L::STAGE_BYTES);
+          tma_load_2d(dst, &map_a, g * BK, tm * BM, &full_bar[s]);
+          tma_load_2d(dst + L::A_BYTES, &map_w, g * BK, tn * BN, &full_bar[s]);
         }
       }
-      if (rank == 0) mbar_drain(full_bar, STAGES, it);   // (a pair's second CTA stays until the first is done)
-    } else if (warp == 1 && rank == 0) {
+      mbar_drain(full_bar, STAGES, it);
+    } else if (warp == 1) {
       // ---------------- MMA issuer (warp-wide loop, one elected lane issues)
-      const uint32_t idesc = instr_desc_e4m3(TILE_M, BN);
+      const uint32_t idesc = instr_desc_e4m3(BM, BN);
       const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
       const uint32_t lo0 = smem_desc_sw128_lo(smem_u32(smem));
       int it = 0;
       bool ok = true;
-      for (int t = first_tile; t < n_tiles && ok; t += tile_step)
+      for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x)
         for (int g = 0; g < p.groups; ++g, ++it) {
           const int s = it % STAGES, buf = it % ACCS;
-          ok = mbar_wait(&acc_empty[buf], ((it / ACCS) & 1) ^ 1, abort_flag) && mbar_wait(&full_bar[s], (it / STAGES) & 1, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
+          ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((it / ACCS) & 1) ^ 1, abort_flag) && mbar_wait(&full_bar[s], (it / STAGES) & 1, abort_flag));
           if (!ok) break;
           tc_fence_after();
           const uint32_t a_lo = lo0 + s * (L::STAGE_BYTES >> 4), b_lo = a_lo + (L::A_BYTES >> 4);
           if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < BK / UMMA_K; ++k) {
-              if (PAIR) umma_fp8_pair_lo(tmem_u + buf * BN, a_lo + (k * UMMA_K >> 4), b_lo + (k * UMMA_K >> 4), idesc, k > 0 ? 1u : 0u);
-              else umma_fp8_lo(tmem_u + buf * BN, a_lo + (k * UMMA_K >> 4), b_lo + (k * UMMA_K >> 4), idesc, k > 0 ? 1u : 0u);
-            }
-            if (PAIR) { umma_commit_pair(&empty_bar[s]); umma_commit_pair(&acc_full[buf]); }
-            else { umma_commit(&empty_bar[s]); umma_commit(&acc_full[buf]); }
+            for (int k = 0; k < BK / UMMA_K; ++k)
+              umma_fp8_lo(tmem_u + buf * BN, a_lo + (k * UMMA_K >> 4), b_lo + (k * UMMA_K >> 4), idesc, k > 0 ? 1u : 0u);
+            umma_commit(&empty_bar[s]);
+            umma_commit(&acc_full[buf]);
           }
           __syncwarp();
         }
@@ -333,10 +276,10 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     auto column = [&](int c) { return GATED ? part * 32 + 128 * c : part * COLS + 32 * c; };
     int it = 0;
     bool ok = true;
-    for (int t = first_tile; t < n_tiles; t += tile_step) {
+    for (int t = blockIdx.x; t < n_tiles; t += gridDim.x) {
       int tm, tile_n;
       tile_at(t, tm, tile_n);
-      const int m = tm * TILE_M + rank * BM + row;
+      const int m = tm * BM + row;
       // the row's scales, four groups to a word where the rows allow it
       const uint8_t* sa = p.a_scales + (long long)min(m, p.m - 1) * p.lda_s;
       auto four_scales = [&](int g) -> uint32_t {
@@ -373,10 +316,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
           if (c == CHUNKS - 1) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
-              if (PAIR) mbar_arrive_cluster(cluster_addr(&acc_empty[buf], 0));
-              else mbar_arrive(&acc_empty[buf]);
-            }
+            if (lane == 0) mbar_arrive(&acc_empty[buf]);
           }
           const float s = GATED && c > 0 ? s1 : s0;
 #pragma unroll
@@ -432,11 +372,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   }
   tc_fence_before();
   __syncthreads();
-  if (PAIR) cluster_sync_all();    // the pair's products have been read, no copy or arrival is under way
-  if (warp == 1) {
-    if (PAIR) tmem_dealloc_pair(tmem_base, 512);
-    else tmem_dealloc(tmem_base, 512);
-  }
+  if (warp == 1) tmem_dealloc(tmem_base, 512);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -720,13 +656,13 @@ static bool make_map(CUtensorMap* map, const void* ptr, int rows, int k, long lo
   return true;
 }
 
-template <int BN, int STAGES, bool GATED, bool PAIR>
+template <int BN, int STAGES, bool GATED>
 static int launch_tiles(const Fp8Args& p, const void* a, long long lda, const void* w, long long ldw, int w_rows, int k, int* status, cudaStream_t s) {
-  using L = Smem<BN, STAGES, PAIR>;
-  auto kern = linear_fp8_kernel<BN, STAGES, GATED, PAIR>;
+  using L = Smem<BN, STAGES>;
+  auto kern = linear_fp8_kernel<BN, STAGES, GATED>;
   TLLM_RESERVE_SMEM("linear_fp8", L::TOTAL, kern);
   CUtensorMap ma, mw;
-  if (!make_map(&ma, a, p.m, k, lda, BM) || !make_map(&mw, w, w_rows, k, ldw, PAIR ? BN / 2 : BN)) TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: cannot describe the operands to the copy unit");
+  if (!make_map(&ma, a, p.m, k, lda, BM) || !make_map(&mw, w, w_rows, k, ldw, BN)) TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: cannot describe the operands to the copy unit");
   // the registers that the summing warpgroups ask for are those of the launch, or they would wait for good
   static int regs = 0;
   if (regs == 0) {
@@ -735,31 +671,11 @@ static int launch_tiles(const Fp8Args& p, const void* a, long long lda, const vo
     regs = fa.numRegs;
   }
   TLLM_REQUIRE(regs * THREADS >= 32 * FIRST_SUM_WARP * REGS_OTHERS + 32 * SUM_WARPS * REGS_SUMS, "linear_fp8: built with %d registers, too few for its split", regs);
-  constexpr int TILE_M = PAIR ? 2 * BM : BM;
-  const int tiles = ((p.m + TILE_M - 1) / TILE_M) * (GATED ? (p.n + 127) / 128 : (p.n + BN - 1) / BN);
+  const int tiles = ((p.m + BM - 1) / BM) * (GATED ? (p.n + 127) / 128 : (p.n + BN - 1) / BN);
   int dev = 0, sm_count = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sm_count < 1)
     TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: cannot read the number of SMs");
-  if (!PAIR) {
-    TLLM_LAUNCH("linear_fp8", kern, tiles < sm_count ? tiles : sm_count, THREADS, L::TOTAL, s, ma, mw, p, status);
-    return TLLM_OK;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * (tiles < sm_count / 2 ? tiles : sm_count / 2));
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = L::TOTAL;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ma, mw, p, status);
-  if (e != cudaSuccess) TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: %s", cudaGetErrorString(e));
+  TLLM_LAUNCH("linear_fp8", kern, tiles < sm_count ? tiles : sm_count, THREADS, L::TOTAL, s, ma, mw, p, status);
   return TLLM_OK;
 }
 
@@ -836,12 +752,7 @@ extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
     TLLM_FEW(128, 6, false, 4);
   }
 #undef TLLM_FEW
-#define TLLM_TILES(BN, STAGES, GATED, PAIR) return launch_tiles<BN, STAGES, GATED, PAIR>(p, a, lda, w, ldw, w_rows, k, status, s)
-  if (gated) {
-    if (m > 128) TLLM_TILES(256, 6, true, true);
-    TLLM_TILES(256, 4, true, false);
-  }
-  if (p.n > 128 && (long long)((m + 255) / 256) * ((n + 255) / 256) >= 37) TLLM_TILES(256, 6, false, true);
-  TLLM_TILES(128, 6, false, false);
-#undef TLLM_TILES
+  if (gated) return launch_tiles<256, 4, true>(p, a, lda, w, ldw, w_rows, k, status, s);
+  if (p.n > 128 && (long long)((m + 127) / 128) * ((n + 255) / 256) >= 74) return launch_tiles<256, 4, false>(p, a, lda, w, ldw, w_rows, k, status, s);
+  return launch_tiles<128, 6, false>(p, a, lda, w, ldw, w_rows, k, status, s);
 }
