@@ -739,20 +739,27 @@ extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
   TLLM_REQUIRE(mode != OUT_FP8 || p.vec_out, "linear_fp8: rows of 8-bit values start on 16 bytes");
   cudaStream_t s = (cudaStream_t)stream;
   const int w_rows = gated ? 256 * ((n + 127) / 128) : n;
+  const long long w_tiles = (n + 127) / 128;
+  // Few rows of A, or so few tiles that K has to be cut to fill the SMs: the weight's 128 rows as the large side (few).  Otherwise tiles
+  // of 128 x 256 when they fill half the SMs, else of 128 x 128.  us, few / 128 x 128 / 128 x 256 (columns x values of K):
+  //   2,560 x 2,048 of 128 rows 7.5 / 9.6 / 13.4, 256 8.9 / 9.8 / 13.4, 512 13.0 / 10.1 / 13.7, 1,024 25 / 17.4 / 14.3
+  //   4,096 x 4,096 of 256 13.1 / 14.5 / 20, 512 20 / 14.8 / 20, 1,024 40 / 27 / 21
+  //   4,096 x 14,336 of 128 20 / 40 / 53, 256 32 / 40 / 53, 512 58 / 40 / 53, 1,024 116 / 78 / 59
+  // gated, few / 128 x 256: 5,632 x 2,048 of 64 rows 11.0 / 14.8, 128 14.7 / 15.4, 256 29 / 16; 14,336 x 4,096 of 64 24.8 / 27.9, 128 45 / 28
 #define TLLM_FEW(BN, STAGES, GATED, HALVES) return launch_few<BN, STAGES, GATED, HALVES>(p, a, lda, w, ldw, w_rows, k, status, s)
-  if (m <= 128) {
-    if (gated) {
-      if (m <= 16) TLLM_FEW(16, 3, true, 1);
-      if (m <= 32) TLLM_FEW(32, 3, true, 1);
-      TLLM_FEW(64, 5, true, 2);
-    }
-    if (m <= 16) TLLM_FEW(16, 6, false, 1);
-    if (m <= 32) TLLM_FEW(32, 5, false, 1);
-    if (m <= 64) TLLM_FEW(64, 4, false, 2);
-    TLLM_FEW(128, 6, false, 4);
+#define TLLM_TILES(BN, STAGES, GATED) return launch_tiles<BN, STAGES, GATED>(p, a, lda, w, ldw, w_rows, k, status, s)
+  if (gated) {
+    if (m <= 16) TLLM_FEW(16, 3, true, 1);
+    if (m <= 32) TLLM_FEW(32, 3, true, 1);
+    if (m <= 64 || ((m + 63) / 64) * w_tiles <= 148) TLLM_FEW(64, 5, true, 2);
+    TLLM_TILES(256, 4, true);
   }
+  if (m <= 16) TLLM_FEW(16, 6, false, 1);
+  if (m <= 32) TLLM_FEW(32, 5, false, 1);
+  if (m <= 64) TLLM_FEW(64, 4, false, 2);
+  if (((m + 127) / 128) * w_tiles <= 74) TLLM_FEW(128, 6, false, 4);
+  if (((m + 127) / 128) * (long long)((n + 255) / 256) >= 74) TLLM_TILES(256, 4, false);
+  TLLM_TILES(128, 6, false);
 #undef TLLM_FEW
-  if (gated) return launch_tiles<256, 4, true>(p, a, lda, w, ldw, w_rows, k, status, s);
-  if (p.n > 128 && (long long)((m + 127) / 128) * ((n + 255) / 256) >= 74) return launch_tiles<256, 4, false>(p, a, lda, w, ldw, w_rows, k, status, s);
-  return launch_tiles<128, 6, false>(p, a, lda, w, ldw, w_rows, k, status, s);
+#undef TLLM_TILES
 }
