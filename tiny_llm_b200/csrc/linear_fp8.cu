@@ -33,6 +33,7 @@ constexpr int THREADS = 32 * (FIRST_SUM_WARP + SUM_WARPS);
 // Registers: the launch gives 96 to each of 640 threads; the first warpgroup hands most of its own to the four that sum
 // (128 * 32 + 512 * 112 = 640 * 96).
 constexpr int REGS_OTHERS = 32, REGS_SUMS = 112;
+constexpr int STAGING_BYTES = 16 * 32 * 4;     // of shared memory per summing warp, for its stores
 constexpr int BAND = 12;         // row tiles per band of the large products' order
 
 enum Output { OUT_BF16 = 0, OUT_F32 = 1, OUT_ADD = 2, OUT_FP8 = 3 };
@@ -129,52 +130,72 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr, uint32_t rank)
 template <int BN, int STAGES>
 struct Smem {
   static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK, STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int MOST_OFFSET = STAGES * STAGE_BYTES;           // the largest magnitudes of a row's four parts
-  static constexpr int BAR_OFFSET = MOST_OFFSET + 4 * BM * 4;
+  static constexpr int STAGING_OFFSET = STAGES * STAGE_BYTES;        // what the summing warps store passes here, or the largest magnitudes
+  static constexpr int BAR_OFFSET = STAGING_OFFSET + SUM_WARPS * STAGING_BYTES;                                      // of a row's four parts
   static constexpr int ACCS = 512 / BN;            // accumulators in tensor memory: the products run that many groups ahead of the sums
   static constexpr int TOTAL = BAR_OFFSET + (2 * STAGES + 2 * ACCS) * 8 + 16 + 1024;
 };
 
 // eight columns as bfloat16
-__device__ __forceinline__ uint4 pack8_bf16(const float* v) {
+__device__ __forceinline__ uint4 pack8_bf16(float4 a, float4 b) {
   uint4 pk;
   __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&pk);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+  h[0] = __floats2bfloat162_rn(a.x, a.y); h[1] = __floats2bfloat162_rn(a.z, a.w);
+  h[2] = __floats2bfloat162_rn(b.x, b.y); h[3] = __floats2bfloat162_rn(b.z, b.w);
   return pk;
 }
 
-// `N` columns of this thread's row from column `n` on, as `mode` says
-template <int N>
-__device__ __forceinline__ void store_columns(const Fp8Args& p, int m, int n, const float* v, int mode) {
-  if (m >= p.m || n >= p.n) return;
-  const bool full = n + N <= p.n && p.vec_out;
-  if (mode == OUT_BF16) {
-    __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + (size_t)m * p.ldo + n;
-    if (full) {
+// A warp's 32 rows (lane l has row m0 + l) of 32 columns from `n` on leave as `mode` says.  They pass through 2 KB of the warp's own in
+// shared memory, 16 rows at a time, so that a store of the warp covers 64 or 128 neighbouring bytes of few rows: straight from the
+// registers every store touched 32 rows, and with rows that do not start on 16 bytes, value by value, that took longer than the products
+// (8,192 rows of 300 x 4,096: 56 us).
+__device__ __forceinline__ void store_columns(const Fp8Args& p, float* staging, int m0, int n, const float* v, int mode) {
+  const int lane = threadIdx.x & 31;
+  const bool vec = p.vec_out && n + 32 <= p.n;
+  // 16 bytes c of row r lie at place c ^ (r % 8) of the row's eight
+  auto place = [&](int r, int c) { return reinterpret_cast<float4*>(staging + r * 32) + (c ^ (r & 7)); };
+#pragma unroll 1
+  for (int r0 = 0; r0 < 32; r0 += 16) {
+    __syncwarp();
+    if ((lane & 16) == r0) {
 #pragma unroll
-      for (int j = 0; j < N; j += 8) *reinterpret_cast<uint4*>(dst + j) = pack8_bf16(v + j);
-    } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (n + j < p.n) dst[j] = __float2bfloat16_rn(v[j]);
+      for (int c = 0; c < 8; ++c) *place(lane & 15, c) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
     }
-  } else {
-    float* dst = reinterpret_cast<float*>(p.out) + (size_t)m * p.ldo + n;
-    if (full) {
+    __syncwarp();
+    if (vec && mode == OUT_BF16) {
 #pragma unroll
-      for (int j = 0; j < N; j += 4) {
-        float4 o = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-        if (mode == OUT_ADD) {
-          const float4 r = *reinterpret_cast<const float4*>(dst + j);
-          o.x += r.x; o.y += r.y; o.z += r.z; o.w += r.w;
-        }
-        *reinterpret_cast<float4*>(dst + j) = o;
+      for (int i = 0; i < 2; ++i) {
+        const int r = 8 * i + lane / 4, c = lane % 4, m = m0 + r0 + r;
+        const uint4 pk = pack8_bf16(*place(r, 2 * c), *place(r, 2 * c + 1));
+        if (m < p.m) *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.out) + (size_t)m * p.ldo + n + 8 * c) = pk;
+      }
+    } else if (vec) {
+      float4 o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int m = m0 + r0 + 4 * i + lane / 8;
+        if (mode == OUT_ADD && m < p.m) o[i] = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(p.out) + (size_t)m * p.ldo + n + 4 * (lane % 8));
+        else o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 4 * i + lane / 8, m = m0 + r0 + r;
+        const float4 x = *place(r, lane % 8);
+        o[i].x += x.x; o[i].y += x.y; o[i].z += x.z; o[i].w += x.w;
+        if (m < p.m) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + (size_t)m * p.ldo + n + 4 * (lane % 8)) = o[i];
       }
     } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (n + j < p.n) dst[j] = mode == OUT_ADD ? dst[j] + v[j] : v[j];
+#pragma unroll 4
+      for (int r = 0; r < 16; ++r) {
+        const int m = m0 + r0 + r;
+        const float x = reinterpret_cast<float*>(place(r, lane / 4))[lane % 4];
+        if (m < p.m && n + lane < p.n) {
+          const size_t at = (size_t)m * p.ldo + n + lane;
+          if (mode == OUT_BF16) reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(x);
+          else if (mode == OUT_ADD) reinterpret_cast<float*>(p.out)[at] += x;
+          else reinterpret_cast<float*>(p.out)[at] = x;
+        }
+      }
     }
   }
 }
@@ -187,7 +208,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
   constexpr int ACCS = L::ACCS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint32_t* most = reinterpret_cast<uint32_t*>(smem + L::MOST_OFFSET);
+  uint32_t* most = reinterpret_cast<uint32_t*>(smem + L::STAGING_OFFSET);
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::BAR_OFFSET);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* acc_full = empty_bar + STAGES;      // accumulator b holds a group's products
@@ -273,6 +294,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     constexpr int COLS = BN / 4, CHUNKS = COLS / 32;
     const int quad = warp & 3, part = (warp - FIRST_SUM_WARP) >> 2;
     const int row = quad * 32 + lane;
+    float* staging = reinterpret_cast<float*>(smem + L::STAGING_OFFSET) + (warp - FIRST_SUM_WARP) * (STAGING_BYTES / 4);
     auto column = [&](int c) { return GATED ? part * 32 + 128 * c : part * COLS + 32 * c; };
     int it = 0;
     bool ok = true;
@@ -331,13 +353,13 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       if (!sums_all(ok)) break;
       if (!GATED) {
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) store_columns<32>(p, m, tile_n * BN + column(c), acc + 32 * c, p.mode);
+        for (int c = 0; c < CHUNKS; ++c) store_columns(p, staging, m - lane, tile_n * BN + column(c), acc + 32 * c, p.mode);
       } else {
         const int n = tile_n * 128 + part * 32;
 #pragma unroll
         for (int j = 0; j < 32; ++j) acc[j] = n + j < p.n ? gate_f(acc[j], acc[32 + j], p.gate) : 0.f;
         if (p.mode != OUT_FP8) {
-          store_columns<32>(p, m, n, acc, OUT_BF16);
+          store_columns(p, staging, m - lane, n, acc, OUT_BF16);
         } else {
           uint32_t largest = 0u;
 #pragma unroll
@@ -569,6 +591,7 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   if (f.slices > 1) cluster_sync_all();
   const uint32_t base = smem_u32(parked);
   const int tokens = min(BN, p.m - m0);
+#pragma unroll 2
   for (int j = rank + f.slices * warp; j < tokens; j += f.slices * WARPS) {
     const int m = m0 + j, n = tile * 128 + 4 * lane;
     float4 part[TILES][8];
