@@ -121,3 +121,34 @@ def test_products_that_do_not_fit(no_device):
         with pytest.raises(KernelError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+# ---------------------------------------------------------------------------------------------- models
+
+
+def test_the_engine_refuses_what_has_no_8_bit_form():
+    from conftest import TINY_A
+    from tiny_llm_b200.config import LlamaConfig, config_from_dict
+    from tiny_llm_b200.engine.loading import parse_weights
+    from tiny_llm_b200.parts import DecoderModel
+    import dunelix_util
+
+    assert parse_weights(None, torch.float32) is False and parse_weights("fp8", torch.bfloat16) is True
+    for weights, dtype in (("fp8", torch.float32), ("int4", torch.bfloat16)):
+        with pytest.raises(ValueError):
+            parse_weights(weights, dtype)
+    model = DecoderModel(LlamaConfig.from_dict(TINY_A).model_spec())
+    with pytest.raises(RuntimeError, match="no weights"):
+        model.to_fp8()
+    model.load({n: torch.zeros([s or 1 for s in w.shape]) for n, w in model.weight_specs().items()})
+    with pytest.raises(ValueError, match="bfloat16 engine"):
+        model.to_fp8()
+    other = DecoderModel(config_from_dict(next(v for v in vars(dunelix_util).values() if isinstance(v, dict) and v.get("architecture") == "Dunelix")).model_spec())
+    other.loaded = True
+    with pytest.raises(ValueError, match="without an 8-bit form"):
+        other.to_fp8()
+
+
+def test_the_command_line_takes_the_form_of_the_weights():
+    from tiny_llm_b200.__main__ import parse_flags
+    assert parse_flags(["--weights=fp8"])["weights"] == "fp8" and parse_flags([])["weights"] == ""

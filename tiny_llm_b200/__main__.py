@@ -1,7 +1,7 @@
 """Command line in the manner of the reference's main.cpp (flags at main.cpp:7-19, loop at :55-81):
 
     python -m tiny_llm_b200 --model_path=DIR [--device=0] [--max_new_tokens=256] [--do_sample=true]
-        [--temperature=0.7] [--top_k=50] [--top_p=0.95] [--page_mode] [--dtype=bfloat16] [--seed=0]
+        [--temperature=0.7] [--top_k=50] [--top_p=0.95] [--page_mode] [--dtype=bfloat16] [--weights=fp8] [--seed=0]
         [--page_size=16] [--num_pages=N | --max_tokens=N] [--max_requests=4] [--max_tokens_per_step=2048]
         [--chunk=512] [--prompt_per_line]
     python -m tiny_llm_b200 --random_weights --config=CONFIG.json [--seed=0] ...
@@ -30,6 +30,7 @@ FLAGS = {
     "top_p": (float, 0.95, "Sample from the smallest set of tokens whose cumulative probability > p"),
     "page_mode": (bool, True, "Paged attention (always on; accepted for compatibility)"),
     "dtype": (str, "bfloat16", "bfloat16 (serving kernels) or float32 (everything in true 32-bit)"),
+    "weights": (str, "", "fp8: the layers' matrices in 8 bits (bfloat16 engine); empty: as --dtype says"),
     "seed": (int, 0, "Seed of the sampler's random stream"),
     "page_size": (int, 16, "Tokens per cache page"),
     "max_tokens": (int, 0, "Tokens the cache pool holds (0: max_requests x the model's positions)"),
@@ -123,7 +124,7 @@ def main(argv=None) -> int:
             scratch = tempfile.TemporaryDirectory(prefix="tiny_llm_random_")
             model_path = write_random_model(scratch.name, load_config(f["config"]), seed=f["seed"], dtype=torch.float32)
         max_tokens = f["max_tokens"] or f["num_pages"] * f["page_size"] or None
-        pipeline = Pipeline(model_path, dtype=f["dtype"], device=f["device"], page_size=f["page_size"],
+        pipeline = Pipeline(model_path, dtype=f["dtype"], weights=f["weights"] or None, device=f["device"], page_size=f["page_size"],
                             max_tokens=max_tokens, max_requests=f["max_requests"],
                             max_tokens_per_step=f["max_tokens_per_step"], chunk=f["chunk"] or None)
         print("\n>>> [Page Mode] Interactive Mode (Multi-line enabled) <<<")

@@ -24,12 +24,25 @@ def parse_dtype(name) -> torch.dtype:
     return DTYPES[name]
 
 
-def load_model(model_dir: str, dtype, device="cuda:0"):
-    """Reads config.json, picks the model by its architecture name, loads the weights by name."""
+def parse_weights(weights, dtype: torch.dtype) -> bool:
+    """Whether the layers' matrices are to be turned to 8 bits: `weights` is None (as the engine's dtype) or "fp8"."""
+    if weights not in (None, "", "fp8"):
+        raise ValueError(f"unknown form of weights {weights!r}; choose fp8, or none for the engine's dtype")
+    if weights and dtype != torch.bfloat16:
+        raise ValueError(f"8-bit weights are for the bfloat16 engine, not {dtype}")
+    return bool(weights)
+
+
+def load_model(model_dir: str, dtype, device="cuda:0", weights=None):
+    """Reads config.json, picks the model by its architecture name, loads the weights by name.  weights="fp8": the layers'
+    matrices are turned to 8 bits when they are loaded (DecoderModel.to_fp8)."""
     dtype = parse_dtype(dtype)
+    fp8 = parse_weights(weights, dtype)
     config = load_config(model_dir)
     model = DecoderModel(config.model_spec())
     model.load(load_state(model.weight_specs(), model_dir, dtype, device, ignore=model.spec.ignored_weights))
+    if fp8:
+        model.to_fp8()
     return config, model
 
 

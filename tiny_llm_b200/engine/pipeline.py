@@ -11,7 +11,7 @@ from typing import Dict, Hashable, List, Optional, Sequence
 import torch
 
 from ..sampling import Sampler, SamplingParams
-from .loading import load_model, make_runner, parse_dtype
+from .loading import load_model, make_runner, parse_dtype, parse_weights
 from .scheduler import PENDING, RUNNING, Request, Scheduled, Scheduler
 from .step import StepEntry
 
@@ -27,12 +27,13 @@ class _Pending:
 class Pipeline:
     def __init__(self, model_path: str, dtype="bfloat16", device: int = 0, page_size: int = 16,
                  max_tokens: Optional[int] = None, max_requests: int = 64, max_tokens_per_step: int = 2048,
-                 chunk: Optional[int] = None, max_positions: Optional[int] = None):
+                 chunk: Optional[int] = None, max_positions: Optional[int] = None, weights: Optional[str] = None):
         """`max_tokens`: tokens the cache pool holds (default: max_requests x the model's positions,
         capped at 1M tokens).  `max_positions`: the longest request (default: the model's own limit, or what the
         pool holds if that is less).  `chunk`: the largest portion of one prompt in one step (default: the step's whole
         token budget; measured at the TinyLlama sizes a step of 512 prompt tokens runs at 233,000 tokens a second and a
-        step of 2,048 at 448,000, so a prompt is cut no finer than the budget asks)."""
+        step of 2,048 at 448,000, so a prompt is cut no finer than the budget asks).  `weights`="fp8": the layers' matrices in 8 bits, for the
+        bfloat16 engine and models whose parts have an 8-bit form (the Llama decoder)."""
         if not chunk:
             chunk = max_tokens_per_step
         if not torch.cuda.is_available():
@@ -42,8 +43,10 @@ class Pipeline:
         self.dtype = parse_dtype(dtype)
         if isinstance(model_path, tuple):   # (config, loaded model): see from_model
             self.config, self.model = model_path
+            if parse_weights(weights, self.dtype):
+                self.model.to_fp8()
         else:
-            self.config, self.model = load_model(model_path, self.dtype, self.device)
+            self.config, self.model = load_model(model_path, self.dtype, self.device, weights=weights)
         spec = self.model.spec
         if max_tokens is None:
             max_tokens = min(max_requests * spec.max_positions, 1 << 20)

@@ -1515,6 +1515,20 @@ def fp8_weight(n: int, k: int, device):
     return data, torch.empty(_fp8_groups(n), _fp8_groups(k), dtype=torch.float32, device=device)
 
 
+def fp8_workspace(workspace, name: str, m: int, k: int):
+    """`fp8_rows` out of a step's workspace."""
+    g = _fp8_groups(k)
+    data, scales = workspace.get(name, (m, -(-k // 16) * 16), FP8), workspace.get(name + "_scales", (m, -(-g // 16) * 16), FP8_SCALE)
+    return data[:, :k], scales[:, :g]
+
+
+def weight_to_fp8(w: torch.Tensor):
+    """(values, scales) of a weight in 8 bits."""
+    out = fp8_weight(w.shape[0], w.shape[1], w.device)
+    quantize_weight_fp8(w, *out)
+    return out
+
+
 # The arguments of an entry point travel as one packed struct, in the order and with the types of its C declaration (P: pointer,
 # q: 64 bits, i: 32 bits, f: float): a call of a dozen ctypes objects takes longer than the small kernels.
 _FP8_ENTRIES = {name: (library, struct.Struct(layout)) for name, library, layout in (

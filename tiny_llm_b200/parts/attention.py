@@ -45,6 +45,7 @@ class GQAttention:
         self.qkv_dim = self.q_dim if shares_cache else self.q_dim + 2 * self.kv_dim
         self.w_qkv = None
         self.w_o = None
+        self.fp8 = False      # True: both matrices are (values, scales) in 8 bits, and `forward` takes 8-bit rows
 
     def cache_need(self):
         return None if self.shares_cache else KVNeed(self.num_kv_heads, self.head_dim, self.window)
@@ -67,19 +68,26 @@ class GQAttention:
         self.w_o = weights[prefix + "o_proj.weight"]
         self.position.prepare(self.w_o.device)
 
+    def to_fp8(self) -> None:
+        """Turns the loaded matrices to 8 bits; queries, keys, values and the cache stay in the engine's dtype."""
+        self.w_qkv, self.w_o = ops.weight_to_fp8(self.w_qkv), ops.weight_to_fp8(self.w_o)
+        self.fp8 = True
+
     def forward(self, ctx, h, resid, cache) -> None:
-        t = h.shape[0]
+        t = h[0].shape[0] if self.fp8 else h.shape[0]
         qkv = ctx.workspace.get("qkv", (t, self.qkv_dim), ctx.dtype)
         pos = self.position
         fused = getattr(pos, "fused", False)
         kv_slots = None if self.shares_cache else cache.slot_mapping
-        if fused and ops.fused_qkv_preferred(t, self.qkv_dim, h.shape[1]) and ops.linear_rope_kv(
+        if not self.fp8 and fused and ops.fused_qkv_preferred(t, self.qkv_dim, h.shape[1]) and ops.linear_rope_kv(
                 h, self.w_qkv, qkv, ctx.batch.positions, pos.cos, pos.sin, self.num_heads, self.num_kv_heads,
                 self.head_dim, cache.k, cache.v, kv_slots):
             pass    # projection, rotation and cache write were one kernel
         else:
             acc = None
-            if fused and ops.prefers_split(h, self.w_qkv):
+            if self.fp8:
+                ops.linear_fp8(*h, *self.w_qkv, qkv)
+            elif fused and ops.prefers_split(h, self.w_qkv):
                 # few rows: K is split over the SMs into a zeroed float32 buffer that the rotate-and-cache kernel consumes
                 acc = ctx.workspace.get_zeroed("qkv_f32", (t, self.qkv_dim))
                 ops.linear(h, self.w_qkv, acc, accumulate=True)
@@ -98,6 +106,11 @@ class GQAttention:
         out = ctx.workspace.get("attn_out", (t, self.q_dim), ctx.dtype)
         ops.paged_attention(qkv, self.num_heads, self.num_kv_heads, self.head_dim, cache.k, cache.v,
                             cache.block_table, ctx.batch, out, self.scale, self.window, ctx.workspace)
+        if self.fp8:
+            rows = ops.fp8_workspace(ctx.workspace, "attn_out_fp8", t, self.q_dim)
+            ops.quantize_fp8(out, *rows)
+            ops.linear_fp8(*rows, *self.w_o, resid, accumulate=True)
+            return
         ops.linear(out, self.w_o, resid, accumulate=True)
 
 

@@ -62,6 +62,7 @@ class SwiGLU:
         self.block = gate_up_block(intermediate_size)
         self.w_gate_up = None
         self.w_down = None
+        self.fp8 = False      # True: both matrices are (values, scales) in 8 bits, and `forward` takes 8-bit rows
 
     def weight_specs(self, prefix: str):
         i, h = self.intermediate_size, self.hidden_size
@@ -74,7 +75,21 @@ class SwiGLU:
         self.w_gate_up = interleave_gate_up(weights[prefix + g], weights[prefix + u], self.block)
         self.w_down = scaled_matrix(weights[prefix + d], self.out_scale)
 
+    def to_fp8(self) -> None:
+        """Turns the loaded matrices to 8 bits.  Gate and up alternate in blocks of 128 rows there, whatever the sizes: the last
+        block of each is filled with zero rows."""
+        rows, pad = self.w_gate_up.view(-1, 2, self.block, self.hidden_size), -self.intermediate_size % ops.FP8_GROUP
+        gate, up = (torch.nn.functional.pad(rows[:, side].reshape(self.intermediate_size, -1), (0, 0, 0, pad)) for side in (0, 1))
+        self.w_gate_up = ops.weight_to_fp8(interleave_gate_up(gate, up, ops.FP8_GROUP))
+        self.w_down = ops.weight_to_fp8(self.w_down)
+        self.fp8 = True
+
     def forward(self, ctx, h, resid) -> None:
+        if self.fp8:
+            act = ops.fp8_workspace(ctx.workspace, "ffn_act_fp8", h[0].shape[0], self.intermediate_size)
+            ops.linear_swiglu_fp8(*h, *self.w_gate_up, *act, act=self.act, limit=self.limit)
+            ops.linear_fp8(*act, *self.w_down, resid, accumulate=True)
+            return
         t = h.shape[0]
         act = ctx.workspace.get("ffn_act", (t, self.intermediate_size), ctx.dtype)
         ops.linear_swiglu(h, self.w_gate_up, act, self.block, ctx.workspace, act=self.act, limit=self.limit)

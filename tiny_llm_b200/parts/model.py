@@ -56,11 +56,21 @@ class Block:
             self.norm2.load(n2, weights)
             self.ffn.load(ff, weights)
 
+    def has_fp8(self) -> bool:
+        """Whether every part that reads or writes rows of the branches has an 8-bit form."""
+        return all(hasattr(n, "forward_fp8") for n in (self.norm1, self.norm2) if n is not None) and \
+            all(hasattr(x, "to_fp8") for x in (self.mixer, self.ffn) if x is not None)
+
+    def to_fp8(self) -> None:
+        for x in (self.mixer, self.ffn):
+            if x is not None:
+                x.to_fp8()
+
     def forward(self, ctx, resid, cache) -> None:
-        h = self.norm1.forward(ctx, resid)
+        h = self.norm1.forward_fp8(ctx, resid) if getattr(self.mixer, "fp8", False) else self.norm1.forward(ctx, resid)
         self.mixer.forward(ctx, h, resid, cache)
         if self.ffn is not None:
-            h = self.norm2.forward(ctx, resid)
+            h = self.norm2.forward_fp8(ctx, resid) if getattr(self.ffn, "fp8", False) else self.norm2.forward(ctx, resid)
             self.ffn.forward(ctx, h, resid)
 
 
@@ -347,6 +357,21 @@ class DecoderModel:
             self.on_logits.load(s.on_logits_name, weights)
         self.lm_head = self.embed if s.tie_word_embeddings else weights[s.lm_head_name]
         self.loaded = True
+
+    def to_fp8(self) -> None:
+        """Turns the matrices of every layer to 8 bits (e4m3 with a scale per block of 128 x 128); from then on their inputs are
+        rounded to 8 bits too, with a scale per row and group of 128.  The embedding table, the output matrix, the norms and
+        the cache stay as they are.  For a loaded bfloat16 model whose parts all have an 8-bit form, before a runner is built."""
+        if not self.loaded:
+            raise RuntimeError("the model has no weights yet")
+        without = [ls.prefix for ls, b in zip(self.spec.layers, self.blocks) if not getattr(b, "has_fp8", bool)()]
+        if without:
+            raise ValueError(f"8-bit weights: layers {without} have parts without an 8-bit form")
+        if self.embed.dtype != torch.bfloat16:
+            raise ValueError(f"8-bit weights are for the bfloat16 engine, not {self.embed.dtype}")
+        for b in self.blocks:
+            if not getattr(b.mixer, "fp8", False):
+                b.to_fp8()
 
     # ---- one step
     def forward(self, ctx) -> torch.Tensor:

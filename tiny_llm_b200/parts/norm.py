@@ -47,6 +47,12 @@ class RMSNorm:
         ops.rms_norm(x, self.weight, self.eps, out, rows)
         return out
 
+    def forward_fp8(self, ctx, x):
+        """`forward` with rows in 8 bits, as (values, scales), for a part whose matrices are in 8 bits."""
+        out = ops.fp8_workspace(ctx.workspace, "norm_fp8", x.shape[0], self.size)
+        ops.rms_norm_fp8(x, self.weight, self.eps, *out)
+        return out
+
 
 class DynamicTanh:
     """Dynamic Tanh: y_j = tanh(alpha x_j) w_j + b_j with one learned number alpha.  It takes the place of a norm and
