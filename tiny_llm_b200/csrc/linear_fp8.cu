@@ -114,18 +114,17 @@ __device__ __forceinline__ bool sums_all(bool ok) {
       : "=r"(r) : "r"((uint32_t)ok), "n"(32 * SUM_WARPS) : "memory");
   return r != 0;
 }
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+// ---- a cluster of CTAs: where `p` of this CTA lies in the CTA of that rank, and a store there that its barrier counts
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
 }
-// four floats at byte address `addr` of this CTA's shared memory, read from the CTA of rank `rank` in the cluster
-__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr, uint32_t rank) {
-  uint32_t remote;
-  float4 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
-  return v;
+__device__ __forceinline__ void st_async_f32(uint32_t addr, float v, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(__float_as_uint(v)), "r"(bar) : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 template <int BN, int STAGES>
 struct Smem {
@@ -399,33 +398,38 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 
 // ---------------------------------------------------------------- few rows
 // Up to 128 rows of A: the weight is the 128-row operand, the rows of A are the BN columns, and K is cut into slices so that every
-// SM streams weights; such a product is bound by reading them once.  The slices of one tile are a thread-block cluster: every CTA
-// adds its groups up in registers (a thread per weight row), leaves the sums in its shared memory, and after a cluster barrier the
-// CTAs share the tile's tokens, a warp per token: it adds the slices over the peers' shared memory in a fixed order, four weight rows
-// per lane, and stores 128 neighbouring columns.  Gated: a CTA has the gate tile and the up tile beside it, two accumulators and four
-// warps for each; the 128 columns that a warp stores are one group of the product behind.
+// SM streams weights; such a product is bound by reading them once, and short ones by the way from the last product to the last store.
+// The slices of one tile are a thread-block cluster, and token j of the tile belongs to CTA j % slices of it.  Every CTA adds its groups
+// up in registers (a thread per weight row) and sends each token's sums to the CTA it belongs to (st.async, counted by a barrier there);
+// that one adds the slices in a fixed order, a warp per token, four weight rows per lane, and stores 128 neighbouring columns.  No CTA
+// waits for the cluster: sums that the owner reads from the others between two cluster barriers took 3,300 cycles from the last sum to
+// the end of the kernel, of 6,100 for one row of 2,560 x 2,048.  Gated: a CTA has the gate tile and the up tile beside it, two
+// accumulators and four warps for each; the 128 columns that a warp stores are one group of the product behind.
 // A tile's columns are dealt to HALVES sets of four summing warps.
 constexpr int FEW_CHUNK = 8;     // groups whose scales (of the row times of the block) are laid out in shared memory at a time
 
-template <int BN, int STAGES, bool GATED, int HALVES>
+template <int BN, int STAGES, bool GATED, int HALVES, bool SLICED>
 struct FewSmem {
   static constexpr int SUM_WARPS = 4 * (GATED ? 2 : 1) * HALVES, THREADS = 64 + 32 * SUM_WARPS;
   static constexpr int TILES = GATED ? 2 : 1, W_BYTES = TILES * 128 * BK, A_BYTES = BN * BK, STAGE_BYTES = W_BYTES + A_BYTES;
-  static constexpr int SCALE_OFFSET = STAGES * STAGE_BYTES;
+  // The sums: [tokens of this CTA][slices][TILES][128 weight rows].  The peers may send theirs while this CTA still works, so they have a
+  // place of their own (whole tokens per CTA: at most 7 more than BN); a CTA without peers leaves them where the stages were.
+  static constexpr int SUMS_OFFSET = SLICED ? STAGES * STAGE_BYTES : 0;
+  static constexpr int SCALE_OFFSET = STAGES * STAGE_BYTES + (SLICED ? (BN + 8) * TILES * 512 : 0);
   static constexpr int BAR_OFFSET = SCALE_OFFSET + TILES * FEW_CHUNK * BN * 4;
-  static constexpr int TOTAL = BAR_OFFSET + (2 * STAGES + 4) * 8 + 16 + 1024;
+  static constexpr int TOTAL = BAR_OFFSET + (2 * STAGES + 5) * 8 + 16 + 1024;
+  static_assert(SLICED || TILES * BN * 512 <= STAGES * STAGE_BYTES, "the sums fit where the stages were");
   static constexpr int RESIDENT = TOTAL <= 113 * 1024 && THREADS <= 320 ? 2 : 1;     // CTAs per SM
-  static_assert(TILES * BN * 128 * 4 <= STAGES * STAGE_BYTES, "the sums are left where the stages were");
 };
 
 struct FewArgs {
   int slices, per_slice;       // slices of K (the cluster), groups per slice (the last may have fewer, or none)
 };
 
-template <int BN, int STAGES, bool GATED, int HALVES>
-__global__ void __launch_bounds__(FewSmem<BN, STAGES, GATED, HALVES>::THREADS, FewSmem<BN, STAGES, GATED, HALVES>::RESIDENT)
+template <int BN, int STAGES, bool GATED, int HALVES, bool SLICED>
+__global__ void __launch_bounds__(FewSmem<BN, STAGES, GATED, HALVES, SLICED>::THREADS, FewSmem<BN, STAGES, GATED, HALVES, SLICED>::RESIDENT)
 linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const Fp8Args p, const FewArgs f, int* __restrict__ status) {
-  using L = FewSmem<BN, STAGES, GATED, HALVES>;
+  using L = FewSmem<BN, STAGES, GATED, HALVES, SLICED>;
   constexpr int TILES = L::TILES, FEW_SUM_WARPS = L::SUM_WARPS, WARPS = 2 + FEW_SUM_WARPS;
   constexpr uint32_t ACC_COLS = TILES * BN, TMEM_COLS = 2 * ACC_COLS < 32 ? 32 : 2 * ACC_COLS;
   extern __shared__ uint8_t smem_raw[];
@@ -435,20 +439,24 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* acc_full = empty_bar + STAGES;
   uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* sums_bar = acc_empty + 2;           // the slices' sums of this CTA's tokens are here
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sums_bar + 1);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  float* parked = reinterpret_cast<float*>(smem);                      // [TILES][BN tokens][128 weight rows] once the stages are done with
+  float* sums = reinterpret_cast<float*>(smem + L::SUMS_OFFSET);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int m0 = blockIdx.x * BN, tile = blockIdx.y, rank = blockIdx.z;
   const int g_begin = min(p.groups, rank * f.per_slice), n_g = min(p.groups, g_begin + f.per_slice) - g_begin;
+  const int tokens = min(BN, p.m - m0), own_tokens = tokens > rank ? (tokens - rank + f.slices - 1) / f.slices : 0;
 
   if (threadIdx.x == 0) {
     tma_prefetch_map(&map_w); tma_prefetch_map(&map_a);
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], FEW_SUM_WARPS); }
+    mbar_init(sums_bar, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (SLICED) mbar_expect_tx(sums_bar, own_tokens * f.slices * TILES * 512);
   }
   if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
   tc_fence_before();
@@ -456,6 +464,7 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
+  if (SLICED) cluster_arrive();        // (waited for below, when everybody has long been here: the peers' barriers are there to be counted on)
   // the weight depends on no earlier kernel: the first stages are asked for before this grid waits for its predecessors
   pdl_trigger();
   const int n_pre = min(n_g, STAGES);
@@ -471,6 +480,8 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   if (warp == 0 && lane == 0)
     for (int i = 0; i < n_pre; ++i) load_weight(i, policy);
   pdl_wait();
+  if (SLICED) cluster_wait();
+  bool ok = true;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -491,7 +502,6 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     const uint32_t idesc = instr_desc_e4m3(128, BN);
     const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
     const uint32_t lo0 = smem_desc_sw128_lo(smem_u32(smem));
-    bool ok = true;
     for (int i = 0; i < n_g; ++i) {
       const int s = i % STAGES, buf = i & 1;
       ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((i >> 1) & 1) ^ 1, abort_flag) && mbar_wait(&full_bar[s], (i / STAGES) & 1, abort_flag));
@@ -531,7 +541,6 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         for (int t = 0; t < TILES; ++t) fetched[q][t] = there ? a * p.w_scales[(long long)(tile * TILES + t) * p.groups + g_begin + i0 + g] : 0.f;
       }
     };
-    bool ok = true;
     fetch(0);
     for (int i0 = 0; i0 < n_g; i0 += FEW_CHUNK) {
       const int n = min(FEW_CHUNK, n_g - i0);
@@ -579,34 +588,40 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
       }
     }
     if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_SUMS); }
-    // the last accumulator is there, so every product has read its stage: the stages are free
-    float* mine = parked + (part * BN + col0) * 128 + row;
+    int owner = col0 % f.slices, place = col0 / f.slices;
 #pragma unroll
-    for (int j = 0; j < COLS; ++j) mine[j * 128] = acc[j];
+    for (int j = 0; j < COLS; ++j) {
+      if (!SLICED) {      // the last accumulator is there, so every product has read its stage: the stages are free
+        sums[((col0 + j) * TILES + part) * 128 + row] = acc[j];
+        continue;
+      }
+      if (col0 + j < tokens)
+        st_async_f32(cluster_addr(sums + ((place * f.slices + rank) * TILES + part) * 128 + row, owner), acc[j], cluster_addr(sums_bar, owner));
+      if (++owner == f.slices) { owner = 0; ++place; }
+    }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
 
-  if (f.slices > 1) cluster_sync_all();
-  const uint32_t base = smem_u32(parked);
-  const int tokens = min(BN, p.m - m0);
-#pragma unroll 2
-  for (int j = rank + f.slices * warp; j < tokens; j += f.slices * WARPS) {
-    const int m = m0 + j, n = tile * 128 + 4 * lane;
+  if (SLICED) cluster_arrive();        // this CTA has sent what it had to
+  const bool here = !SLICED || own_tokens == 0 || mbar_wait(sums_bar, 0, abort_flag);
+  if (!here && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_SUMS); }
+  for (int i = here ? warp : own_tokens; i < own_tokens; i += WARPS) {
+    const int m = m0 + rank + i * f.slices, n = tile * 128 + 4 * lane;
     float4 part[TILES][8];
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
 #pragma unroll
       for (int z = 0; z < 8; ++z)
-        if (z < f.slices) part[t][z] = ld_cluster_f32x4(base + (uint32_t)((t * BN + j) * 128 + 4 * lane) * 4u, z);
+        if (SLICED ? z < f.slices : z == 0) part[t][z] = reinterpret_cast<const float4*>(sums)[((i * f.slices + z) * TILES + t) * 32 + lane];
     float sum[TILES][4];
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
       sum[t][0] = sum[t][1] = sum[t][2] = sum[t][3] = 0.f;
 #pragma unroll
       for (int z = 0; z < 8; ++z)
-        if (z < f.slices) { sum[t][0] += part[t][z].x; sum[t][1] += part[t][z].y; sum[t][2] += part[t][z].z; sum[t][3] += part[t][z].w; }
+        if (SLICED ? z < f.slices : z == 0) { sum[t][0] += part[t][z].x; sum[t][1] += part[t][z].y; sum[t][2] += part[t][z].z; sum[t][3] += part[t][z].w; }
     }
     if (GATED) {
 #pragma unroll
@@ -651,7 +666,11 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
       }
     }
   }
-  if (f.slices > 1) cluster_sync_all();   // no CTA leaves while a peer still reads its shared memory
+  // Everybody has sent (whoever has its sums knows that already).  A CTA that gave up waiting for them stays until they have landed.
+  if (SLICED) {
+    cluster_wait();
+    if (!here) mbar_drain(sums_bar, 1, 1);
+  }
 }
 
 // ---------------------------------------------------------------- host side
@@ -702,19 +721,14 @@ static int launch_tiles(const Fp8Args& p, const void* a, long long lda, const vo
   return TLLM_OK;
 }
 
-template <int BN, int STAGES, bool GATED, int HALVES>
-static int launch_few(const Fp8Args& p, const void* a, long long lda, const void* w, long long ldw, int w_rows, int k, int* status, cudaStream_t s) {
-  using L = FewSmem<BN, STAGES, GATED, HALVES>;
-  auto kern = linear_fp8_few_kernel<BN, STAGES, GATED, HALVES>;
+template <int BN, int STAGES, bool GATED, int HALVES, bool SLICED>
+static int launch_few(const Fp8Args& p, const FewArgs& f, const void* a, long long lda, const void* w, long long ldw, int w_rows, int k, int* status, cudaStream_t s) {
+  using L = FewSmem<BN, STAGES, GATED, HALVES, SLICED>;
+  auto kern = linear_fp8_few_kernel<BN, STAGES, GATED, HALVES, SLICED>;
   TLLM_RESERVE_SMEM("linear_fp8", L::TOTAL, kern);
   CUtensorMap ma, mw;
   if (!make_map(&mw, w, w_rows, k, ldw, 128) || !make_map(&ma, a, p.m, k, lda, BN)) TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: cannot describe the operands to the copy unit");
   const int tiles = (p.n + 127) / 128, row_tiles = (p.m + BN - 1) / BN;
-  // as many slices as the 148 SMs take, eight at most, four groups at least in each
-  FewArgs f;
-  f.slices = max(1, min(min(8, p.groups / 4), 148 * L::RESIDENT / (tiles * row_tiles)));
-  f.per_slice = (p.groups + f.slices - 1) / f.slices;
-  f.slices = (p.groups + f.per_slice - 1) / f.per_slice;
   TLLM_REQUIRE(tiles <= 65535, "linear_fp8: %d columns are too many for one launch", p.n);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(row_tiles, tiles, f.slices);
@@ -733,6 +747,21 @@ static int launch_few(const Fp8Args& p, const void* a, long long lda, const void
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mw, ma, p, f, status);
   if (e != cudaSuccess) TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: %s", cudaGetErrorString(e));
   return TLLM_OK;
+}
+
+// Slices of K for a kernel that fits `resident` CTAs on an SM: as many as the 148 SMs take, eight at most, four groups at least in each.
+static FewArgs few_slices(int ctas, int groups, int resident) {
+  FewArgs f;
+  f.slices = max(1, min(min(8, groups / 4), 148 * resident / ctas));
+  f.per_slice = (groups + f.slices - 1) / f.slices;
+  f.slices = (groups + f.per_slice - 1) / f.per_slice;
+  return f;
+}
+template <int BN, int STAGES, int STAGES_WHOLE, bool GATED, int HALVES>     // (stages with slices, and without)
+static int launch_few_rows(const Fp8Args& p, const void* a, long long lda, const void* w, long long ldw, int w_rows, int k, int* status, cudaStream_t s) {
+  const FewArgs f = few_slices(((p.n + 127) / 128) * ((p.m + BN - 1) / BN), p.groups, FewSmem<BN, STAGES, GATED, HALVES, true>::RESIDENT);
+  if (f.slices > 1) return launch_few<BN, STAGES, GATED, HALVES, true>(p, f, a, lda, w, ldw, w_rows, k, status, s);
+  return launch_few<BN, STAGES_WHOLE, GATED, HALVES, false>(p, f, a, lda, w, ldw, w_rows, k, status, s);
 }
 
 }  // namespace tllm
@@ -769,18 +798,18 @@ extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
   //   4,096 x 4,096 of 256 13.1 / 14.5 / 20, 512 20 / 14.8 / 20, 1,024 40 / 27 / 21
   //   4,096 x 14,336 of 128 20 / 40 / 53, 256 32 / 40 / 53, 512 58 / 40 / 53, 1,024 116 / 78 / 59
   // gated, few / 128 x 256: 5,632 x 2,048 of 64 rows 11.0 / 14.8, 128 14.7 / 15.4, 256 29 / 16; 14,336 x 4,096 of 64 24.8 / 27.9, 128 45 / 28
-#define TLLM_FEW(BN, STAGES, GATED, HALVES) return launch_few<BN, STAGES, GATED, HALVES>(p, a, lda, w, ldw, w_rows, k, status, s)
+#define TLLM_FEW(BN, STAGES, WHOLE, GATED, HALVES) return launch_few_rows<BN, STAGES, WHOLE, GATED, HALVES>(p, a, lda, w, ldw, w_rows, k, status, s)
 #define TLLM_TILES(BN, STAGES, GATED) return launch_tiles<BN, STAGES, GATED>(p, a, lda, w, ldw, w_rows, k, status, s)
   if (gated) {
-    if (m <= 16) TLLM_FEW(16, 3, true, 1);
-    if (m <= 32) TLLM_FEW(32, 3, true, 1);
-    if (m <= 64 || ((m + 63) / 64) * w_tiles <= 148) TLLM_FEW(64, 5, true, 2);
+    if (m <= 16) TLLM_FEW(16, 2, 3, true, 1);
+    if (m <= 32) TLLM_FEW(32, 4, 3, true, 1);
+    if (m <= 64 || ((m + 63) / 64) * w_tiles <= 148) TLLM_FEW(64, 3, 5, true, 2);
     TLLM_TILES(256, 4, true);
   }
-  if (m <= 16) TLLM_FEW(16, 6, false, 1);
-  if (m <= 32) TLLM_FEW(32, 5, false, 1);
-  if (m <= 64) TLLM_FEW(64, 4, false, 2);
-  if (((m + 127) / 128) * w_tiles <= 74) TLLM_FEW(128, 6, false, 4);
+  if (m <= 16) TLLM_FEW(16, 5, 6, false, 1);
+  if (m <= 32) TLLM_FEW(32, 4, 5, false, 1);
+  if (m <= 64) TLLM_FEW(64, 3, 4, false, 2);
+  if (((m + 127) / 128) * w_tiles <= 74) TLLM_FEW(128, 4, 6, false, 4);
   if (((m + 127) / 128) * (long long)((n + 255) / 256) >= 74) TLLM_TILES(256, 4, false);
   TLLM_TILES(128, 6, false);
 #undef TLLM_FEW
