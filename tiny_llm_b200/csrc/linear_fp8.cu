@@ -12,6 +12,7 @@
 //
 // Sizes: any M, N and K; rows of A and W start on 16 bytes.  TMA fills the tails with zeros, the epilogue masks them.  Every wait
 // is bounded: on expiry the kernel records a code in `status`, stops issuing, frees its tensor memory and returns.
+#include <atomic>
 #include <cmath>
 #include <map>
 #include <mutex>
@@ -406,17 +407,16 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 // the end of the kernel, of 6,100 for one row of 2,560 x 2,048.  Gated: a CTA has the gate tile and the up tile beside it, two
 // accumulators and four warps for each; the 128 columns that a warp stores are one group of the product behind.
 // A tile's columns are dealt to HALVES sets of four summing warps.
-constexpr int FEW_CHUNK = 8;     // groups whose scales (of the row times of the block) are laid out in shared memory at a time
-
 template <int BN, int STAGES, bool GATED, int HALVES, bool SLICED>
 struct FewSmem {
   static constexpr int SUM_WARPS = 4 * (GATED ? 2 : 1) * HALVES, THREADS = 64 + 32 * SUM_WARPS;
+  static constexpr int CHUNK = BN >= 64 ? 4 : 8;                      // groups whose scales are laid out in shared memory at a time
   static constexpr int TILES = GATED ? 2 : 1, W_BYTES = TILES * 128 * BK, A_BYTES = BN * BK, STAGE_BYTES = W_BYTES + A_BYTES;
   // The sums: [tokens of this CTA][slices][TILES][128 weight rows].  The peers may send theirs while this CTA still works, so they have a
   // place of their own (whole tokens per CTA: at most 7 more than BN); a CTA without peers leaves them where the stages were.
   static constexpr int SUMS_OFFSET = SLICED ? STAGES * STAGE_BYTES : 0;
   static constexpr int SCALE_OFFSET = STAGES * STAGE_BYTES + (SLICED ? (BN + 8) * TILES * 512 : 0);
-  static constexpr int BAR_OFFSET = SCALE_OFFSET + TILES * FEW_CHUNK * BN * 4;
+  static constexpr int BAR_OFFSET = SCALE_OFFSET + TILES * CHUNK * BN * 4;
   static constexpr int TOTAL = BAR_OFFSET + (2 * STAGES + 5) * 8 + 16 + 1024;
   static_assert(SLICED || TILES * BN * 512 <= STAGES * STAGE_BYTES, "the sums fit where the stages were");
   static constexpr int RESIDENT = TOTAL <= 113 * 1024 && THREADS <= 320 ? 2 : 1;     // CTAs per SM
@@ -430,7 +430,7 @@ template <int BN, int STAGES, bool GATED, int HALVES, bool SLICED>
 __global__ void __launch_bounds__(FewSmem<BN, STAGES, GATED, HALVES, SLICED>::THREADS, FewSmem<BN, STAGES, GATED, HALVES, SLICED>::RESIDENT)
 linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const Fp8Args p, const FewArgs f, int* __restrict__ status) {
   using L = FewSmem<BN, STAGES, GATED, HALVES, SLICED>;
-  constexpr int TILES = L::TILES, FEW_SUM_WARPS = L::SUM_WARPS, WARPS = 2 + FEW_SUM_WARPS;
+  constexpr int FEW_CHUNK = L::CHUNK, TILES = L::TILES, FEW_SUM_WARPS = L::SUM_WARPS, WARPS = 2 + FEW_SUM_WARPS;
   constexpr uint32_t ACC_COLS = TILES * BN, TMEM_COLS = 2 * ACC_COLS < 32 ? 32 : 2 * ACC_COLS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -749,19 +749,58 @@ static int launch_few(const Fp8Args& p, const FewArgs& f, const void* a, long lo
   return TLLM_OK;
 }
 
-// Slices of K for a kernel that fits `resident` CTAs on an SM: as many as the 148 SMs take, eight at most, four groups at least in each.
-static FewArgs few_slices(int ctas, int groups, int resident) {
-  FewArgs f;
-  f.slices = max(1, min(min(8, groups / 4), 148 * resident / ctas));
-  f.per_slice = (groups + f.slices - 1) / f.slices;
-  f.slices = (groups + f.per_slice - 1) / f.per_slice;
-  return f;
+// How many clusters of `slices` CTAs the current device runs side by side: a cluster stays within a group of SMs, so that sizes that do
+// not divide the group leave some of its SMs idle (with a CTA per SM, 74 of two, 45 of three, 33, 26, 22, 15, 15).  Asked once per kernel,
+// size and device.  The answer counts one CTA per SM for kernels that use tensor memory, of which RESIDENT run (296 CTAs of 128 values of
+// K take 3.0 us, 297 4.4).
+template <int BN, int STAGES, bool GATED, int HALVES>
+static int most_clusters(int slices) {
+  using L = FewSmem<BN, STAGES, GATED, HALVES, true>;
+  static std::atomic<int> held[PerDeviceLimit::DEVICES][9] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= PerDeviceLimit::DEVICES) return 0;
+  int n = held[dev][slices].load(std::memory_order_relaxed);
+  if (n > 0) return n - 1;
+  auto kern = linear_fp8_few_kernel<BN, STAGES, GATED, HALVES, true>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL) != cudaSuccess) return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(1, 1, slices);
+  cfg.blockDim = dim3(L::THREADS);
+  cfg.dynamicSmemBytes = L::TOTAL;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = slices;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) return 0;
+  n *= L::RESIDENT;
+  held[dev][slices].store(n + 1, std::memory_order_relaxed);
+  return n;
 }
+
+// Slices of K: as many as leave four groups to each, eight at most, and let all tiles run at once (6,144 x 4,096, 48 tiles: 6 slices in
+// two rounds 9.5 us, 5 in one 6.6; 2,560 x 2,048: 8 slices of two groups 4.0, 4 of four 3.8).  Where the slices are long, a few clusters
+// more than run at once cost less than fewer slices (4,096 x 14,336, 32 tiles: 8 slices of 14 groups, 30 clusters at once, 11.0 us, 6 of
+// 19 12.1).
 template <int BN, int STAGES, int STAGES_WHOLE, bool GATED, int HALVES>     // (stages with slices, and without)
 static int launch_few_rows(const Fp8Args& p, const void* a, long long lda, const void* w, long long ldw, int w_rows, int k, int* status, cudaStream_t s) {
-  const FewArgs f = few_slices(((p.n + 127) / 128) * ((p.m + BN - 1) / BN), p.groups, FewSmem<BN, STAGES, GATED, HALVES, true>::RESIDENT);
-  if (f.slices > 1) return launch_few<BN, STAGES, GATED, HALVES, true>(p, f, a, lda, w, ldw, w_rows, k, status, s);
-  return launch_few<BN, STAGES_WHOLE, GATED, HALVES, false>(p, f, a, lda, w, ldw, w_rows, k, status, s);
+  const long long tiles = ((p.n + 127) / 128) * (long long)((p.m + BN - 1) / BN);
+  FewArgs f;
+  f.slices = min(8, p.groups / 4);
+  for (; f.slices > 1; --f.slices) {
+    const int most = most_clusters<BN, STAGES, GATED, HALVES>(f.slices);
+    if (tiles <= (p.groups >= 12 * f.slices ? most + most / 15 : most)) break;
+  }
+  if (f.slices <= 1) {
+    f.slices = 1;
+    f.per_slice = p.groups;
+    return launch_few<BN, STAGES_WHOLE, GATED, HALVES, false>(p, f, a, lda, w, ldw, w_rows, k, status, s);
+  }
+  f.per_slice = (p.groups + f.slices - 1) / f.slices;
+  f.slices = (p.groups + f.per_slice - 1) / f.per_slice;
+  return launch_few<BN, STAGES, GATED, HALVES, true>(p, f, a, lda, w, ldw, w_rows, k, status, s);
 }
 
 }  // namespace tllm
