@@ -256,3 +256,95 @@ def test_no_rows(ops):
     ops.linear_fp8(*a, *w, torch.empty(0, 256, device=DEV))
     ops.linear_swiglu_fp8(*a, *w, torch.empty(0, 128, dtype=torch.bfloat16, device=DEV))
     assert ops.launches == before
+
+
+# ---------------------------------------------------------------------------------------------- calls
+
+
+def calls(ops, m, n, k):
+    """Every operator once, as (what it leaves, the call)."""
+    g = rng(m + n + k)
+    x, w, norm = randn(g, m, k), randn(g, n, k), 1 + 0.1 * randn(g, k)
+    a, w8, gu = rows8(ops, x), weight8(ops, w), gated_weight(ops, g, n, k)
+    rows, rows_b, weight = ops.fp8_rows(m, k, DEV), ops.fp8_rows(m, k, DEV), ops.fp8_weight(n, k, DEV)
+    f32, bf16, acc, wide = torch.empty(m, n, device=DEV), torch.empty(m, n, dtype=torch.bfloat16, device=DEV), torch.zeros(m, n, device=DEV), torch.zeros(m, n + 9, device=DEV)
+    h, h8 = torch.empty(m, n, dtype=torch.bfloat16, device=DEV), ops.fp8_rows(m, n, DEV)
+    idx = torch.arange(m, dtype=torch.int32, device=DEV).flip(0)
+    return [(rows, lambda: ops.quantize_fp8(x, *rows)), (rows, lambda: ops.quantize_fp8(x.bfloat16(), *rows)), (weight, lambda: ops.quantize_weight_fp8(w, *weight)),
+            (rows_b, lambda: ops.rms_norm_fp8(x, norm, 1e-5, *rows_b)), (rows_b, lambda: ops.rms_norm_fp8(x, norm, 1e-5, *rows_b, rows=idx)),
+            ((f32,), lambda: ops.linear_fp8(*a, *w8, f32)), ((bf16,), lambda: ops.linear_fp8(*a, *w8, bf16)),
+            ((acc,), lambda: ops.linear_fp8(*a, *w8, acc.zero_(), accumulate=True)), ((wide,), lambda: ops.linear_fp8(*a, *w8, wide[:, 4: 4 + n])),
+            ((h,), lambda: ops.linear_swiglu_fp8(*a, *gu, h)), (h8, lambda: ops.linear_swiglu_fp8(*a, *gu, *h8, act="clamped", limit=2.0)),
+            (h8, lambda: ops.linear_swiglu_fp8(*a, *gu, *h8, act="gelu_tanh"))]
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 256, 128), (2, 130, 200), (200, 300, 77)])
+def test_calls_through_the_interpreter_do_the_same(ops, monkeypatch, m, n, k):
+    for left, call in calls(ops, m, n, k):
+        call()                                                       # (the first one loads what there is)
+        assert ops._fp8_native, "the calls' extension was not built"
+        before = ops.launches
+        call()
+        assert ops.launches == before + 1
+        want = [t.contiguous().view(torch.uint8).clone() for t in left]
+        monkeypatch.setattr(ops, "_fp8_native", False)
+        call()
+        assert ops.launches == before + 2
+        monkeypatch.undo()
+        assert all(torch.equal(t.contiguous().view(torch.uint8), v) for t, v in zip(left, want))
+
+
+def test_refused_calls_launch_nothing(ops):
+    g = rng(0)
+    x, a, w = randn(g, 4, 256), ops.fp8_rows(4, 256, DEV), weight8(ops, randn(g, 300, 256))
+    ops.quantize_fp8(x, *a)
+    out, before = torch.full((4, 300), 7.0, device=DEV), ops.launches
+    for call in (lambda: ops.linear_fp8(*a, *w, out[:, :299]), lambda: ops.linear_fp8(a[0][:, 16:], a[1], *w, out), lambda: ops.linear_fp8(*a, *w, out.cpu()),
+                 lambda: ops.linear_fp8(a[0], a[1].float(), *w, out), lambda: ops.linear_fp8(*a, w[0], w[1][:2], out), lambda: ops.linear_fp8(*a, *w, out.half()),
+                 lambda: ops.linear_fp8(*a, *w, out.T), lambda: ops.linear_fp8(*a, *w, out[:1].expand(4, 300)), lambda: ops.linear_fp8(*a, w[0].cpu(), w[1], out),
+                 lambda: ops.linear_fp8(*a, *w, out.bfloat16(), accumulate=True), lambda: ops.linear_swiglu_fp8(*a, *w, out.bfloat16()),
+                 lambda: ops.linear_swiglu_fp8(*a, *weight8(ops, randn(g, 512, 256)), out[:, :256].bfloat16(), act="clamped"),
+                 lambda: ops.quantize_fp8(x[:, :255], *a), lambda: ops.quantize_fp8(x.double(), *a), lambda: ops.quantize_fp8(x, a[0], a[1][:2]),
+                 lambda: ops.quantize_fp8(x.T, *ops.fp8_rows(256, 4, DEV)), lambda: ops.rms_norm_fp8(x, x[0].cpu(), 1e-5, *a),
+                 lambda: ops.rms_norm_fp8(x[:, ::2], x[0, ::2], 1e-5, *ops.fp8_rows(4, 128, DEV)), lambda: ops.quantize_weight_fp8(x, a[0], a[1])):
+        before = ops.launches
+        with pytest.raises(ops.KernelError):
+            call()
+        assert ops.launches <= before + 1      # (some prepare an operand with a launch of their own)
+    assert bool((out == 7.0).all())
+
+
+def test_threads_on_streams_of_their_own(ops):
+    """Two threads at once, each on a stream of its own, with shared weights: what each gets alone."""
+    import threading
+    g = rng(5)
+    w, gu = weight8(ops, randn(g, 500, 512)), gated_weight(ops, g, 300, 512)
+    rows = [rows8(ops, randn(g, m, 512)) for m in (3, 150)]
+    want = []
+    for a in rows:
+        o, h = torch.empty(a[0].shape[0], 500, device=DEV), ops.fp8_rows(a[0].shape[0], 300, DEV)
+        ops.linear_fp8(*a, *w, o)
+        ops.linear_swiglu_fp8(*a, *gu, *h)
+        want.append((o, h[0].float(), h[1].float()))
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                a = rows[i]
+                o, h = torch.empty_like(want[i][0]), ops.fp8_rows(a[0].shape[0], 300, DEV)
+                for _ in range(200):
+                    ops.linear_fp8(*a, *w, o)
+                    ops.linear_swiglu_fp8(*a, *gu, *h)
+                torch.cuda.current_stream().synchronize()
+                got[i] = (o, h[0].float(), h[1].float())
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors
+    assert all(torch.equal(x, y) for p, q in zip(got, want) for x, y in zip(p, q))

@@ -7,6 +7,7 @@ from __future__ import annotations
 import ctypes
 import os
 import struct
+import sys
 from typing import Optional
 
 import torch
@@ -1538,8 +1539,28 @@ _FP8_ENTRIES = {name: (library, struct.Struct(layout)) for name, library, layout
     ("tllm_linear_fp8", "linear_fp8", "PqPqPqPPqPqiiiiiifPP"))}
 _fp8_loaded = {}
 
+# The same calls without the interpreter (csrc/fp8_calls.cpp), for a call whose arguments are all ordinary: None until the first
+# 8-bit launch of the process has loaded it, False where it cannot be built (the calls then go through the functions below, which
+# launch the same kernels; TLLM_NATIVE_CALLS=0 asks for that).  us a call among others, through the functions / without: normed 8 rows
+# of 2,048 6.6 / 3.2, product of one row 2,560 x 2,048 8.5 / 4.0, rows 33 x 2,000 6.2 / 3.2.
+_fp8_native = None if os.environ.get("TLLM_NATIVE_CALLS", "1") != "0" else False
+
+
+def _fp8_load_native() -> None:
+    global _fp8_native
+    try:
+        module = build.load_extension("fp8_calls")
+    except (BuildError, OSError, ImportError) as e:
+        print(f"[tiny_llm_b200] 8-bit calls go through the interpreter: {e}", file=sys.stderr, flush=True)
+        _fp8_native = False
+        return
+    module.bind(*(ctypes.cast(getattr(build.load_library(library), name), ctypes.c_void_p).value for name, (library, _) in _FP8_ENTRIES.items()))
+    _fp8_native = module
+
 
 def _fp8_call(name: str, *args) -> None:
+    if _fp8_native is None:
+        _fp8_load_native()
     got = _fp8_loaded.get(name)
     if got is None:
         library, layout = _FP8_ENTRIES[name]
@@ -1595,6 +1616,12 @@ def _fp8_weight_scales(name: str, t: torch.Tensor, n: int, k: int) -> None:
 def quantize_fp8(x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor) -> None:
     """Rows of bfloat16 or float32 (a slice of wider rows is fine) to 8-bit rows: out e4m3 [M, K], scales e8m0
     [M, ceil(K / 128)], as `fp8_rows` makes them."""
+    global launches
+    if _fp8_native and _tape is None:
+        here = torch._C._cuda_getDevice()
+        if _fp8_native.quantize(x, out, scales, here, torch._C._cuda_getCurrentRawStream(here)):
+            launches += 1
+            return
     here = _fp8_here("quantize_fp8", x, out, scales)
     shape = x.shape
     if len(shape) != 2 or shape != out.shape or (x.stride(1) != 1 and shape[1] > 1):
@@ -1613,6 +1640,12 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: torch.T
                  rows: Optional[torch.Tensor] = None) -> None:
     """`rms_norm` (x and weight float32, statistics in 32 bits) whose rows leave in 8 bits, rounded from 32: out e4m3
     [M, K], scales e8m0 [M, ceil(K / 128)].  `rows` (int32): which rows of x are taken."""
+    global launches
+    if rows is None and _fp8_native and _tape is None:
+        here = torch._C._cuda_getDevice()
+        if _fp8_native.rms_norm(x, weight, eps, out, scales, here, torch._C._cuda_getCurrentRawStream(here)):
+            launches += 1
+            return
     if rows is None:
         here, taken = _fp8_here("rms_norm_fp8", x, weight, out, scales), 0
     else:
@@ -1635,6 +1668,12 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: torch.T
 def quantize_weight_fp8(w: torch.Tensor, out: torch.Tensor, scales: torch.Tensor) -> None:
     """A weight [N, K] of bfloat16 or float32 to 8 bits: out e4m3 [N, K], scales float32 [ceil(N / 128), ceil(K / 128)], one
     per block of 128 x 128, as `fp8_weight` makes them."""
+    global launches
+    if _fp8_native and _tape is None:
+        here = torch._C._cuda_getDevice()
+        if _fp8_native.quantize_weight(w, out, scales, here, torch._C._cuda_getCurrentRawStream(here)):
+            launches += 1
+            return
     here = _fp8_here("quantize_weight_fp8", w, out, scales)
     shape = w.shape
     if len(shape) != 2 or shape != out.shape or (w.stride(1) != 1 and shape[1] > 1):
@@ -1682,6 +1721,14 @@ def linear_fp8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scale
     float32); accumulate=True adds the product into a float32 `out`.  Any M, N and K; rows of a and w start on 16 bytes.
     `w` and its scales are taken for a loaded weight (see `linear`): `quantize_weight_fp8` may come right before, but no
     other launch of this package that still runs may be writing them."""
+    global launches
+    if _fp8_native and _tape is None:
+        here = torch._C._cuda_getDevice()
+        status = _status.get(here)
+        if status is not None and _fp8_native.linear(a, a_scales, w, w_scales, out, accumulate, here, torch._C._cuda_getCurrentRawStream(here),
+                                                     status.data_ptr()):
+            launches += 1
+            return
     here = _fp8_here("linear_fp8", a, a_scales, w, w_scales, out)
     dtype = out.dtype
     if a.dim() != 2 or w.dim() != 2 or out.shape != (a.shape[0], w.shape[0]) or (dtype is not torch.float32 and dtype is not torch.bfloat16):
@@ -1701,6 +1748,15 @@ def linear_swiglu_fp8(a: torch.Tensor, a_scales: torch.Tensor, w_gate_up: torch.
     kernel; act one of GLU_ACTS (`limit` belongs to "clamped").  Wg and Wu [I, K] alternate in `w_gate_up` in blocks of 128 rows,
     zero rows filling the last block of each: 256 * ceil(I / 128) rows.  `out` [M, I] is bfloat16, or e4m3 with e8m0 `out_scales`
     [M, ceil(I / 128)], rounded from 32 bits: what `linear_fp8` reads next."""
+    global launches
+    code = GLU_ACTS.get(act)
+    if _fp8_native and _tape is None and code is not None and (act != "clamped" or limit > 0):
+        here = torch._C._cuda_getDevice()
+        status = _status.get(here)
+        if status is not None and _fp8_native.gated(a, a_scales, w_gate_up, w_scales, out, out_scales, code, limit if act == "clamped" else 0.0,
+                                                    here, torch._C._cuda_getCurrentRawStream(here), status.data_ptr()):
+            launches += 1
+            return
     if out_scales is None:
         here = _fp8_here("linear_swiglu_fp8", a, a_scales, w_gate_up, w_scales, out)
         mode, fits = OUT_SAME, out.dtype is torch.bfloat16
@@ -2067,6 +2123,10 @@ ATTENTION_TALK_DIMS = ((128, 128),)    # (key size, value size) pairs of the mix
 def build_all(verbose: bool = True):
     """Compiles every library (what `__graft_entry__.build()` calls); returns their paths."""
     paths = [build.compile_library(n, verbose=verbose) for n in ALL_LIBRARIES]
+    try:
+        paths.append(build.compile_extension("fp8_calls", verbose=verbose))
+    except BuildError as e:    # (the calls that it shortens work without)
+        print(f"[tiny_llm_b200] {e}", file=sys.stderr, flush=True)
     paths += [build.compile_library("attention_mma", flags=(f"-DTLLM_HEAD_DIM={hd}",), verbose=verbose)
               for hd in ATTENTION_HEAD_DIMS]
     paths += [build.compile_library("attention_tc", flags=(f"-DTLLM_HEAD_DIM={hd}",), verbose=verbose)

@@ -135,6 +135,48 @@ def load_library(name: str, extra_headers=(), flags=()) -> ctypes.CDLL:
         return lib
 
 
+def compile_extension(name: str, verbose: bool = True) -> str:
+    """Compiles csrc/<name>.cpp, a Python extension that reads torch tensors, with the host compiler if no current object exists;
+    returns the object's path.  Raises BuildError where the compiler or Python's headers are missing."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    include = sysconfig.get_paths()["include"]
+    flags = ["-O2", "-std=c++17", "-shared", "-fPIC", "-I", os.path.join(root, "include"), "-I", include]
+    source = os.path.join(CSRC, name + ".cpp")
+    h = hashlib.sha256()
+    with open(source, "rb") as fh:
+        h.update(fh.read())
+    h.update(" ".join(flags + [torch.__version__, sys.version]).encode())
+    out = os.path.join(build_dir(), f"{name}-{h.hexdigest()[:16]}.so")
+    if os.path.isfile(out):
+        return out
+    compiler = shutil.which(os.environ.get("CXX") or "g++")
+    if compiler is None or not os.path.isfile(os.path.join(include, "Python.h")):
+        raise BuildError(f"{name}.cpp needs a C++ compiler and Python's headers")
+    tmp = f"{out}.{os.getpid()}.tmp"
+    if verbose:
+        print(f"[tiny_llm_b200] compiling {name}.cpp ...", file=sys.stderr, flush=True)
+    lib = os.path.join(root, "lib")
+    proc = subprocess.run([compiler] + flags + ["-o", tmp, source, "-L", lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", f"-Wl,-rpath,{lib}"],
+                          stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if proc.returncode != 0:
+        raise BuildError(f"the host compiler failed on {name}.cpp:\n{proc.stdout}")
+    os.replace(tmp, out)
+    return out
+
+
+def load_extension(name: str):
+    """The Python module of csrc/<name>.cpp."""
+    import importlib.machinery
+    import importlib.util
+    loader = importlib.machinery.ExtensionFileLoader(name, compile_extension(name))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader(name, loader))
+    loader.exec_module(module)
+    return module
+
+
 def _pdl_default() -> bool:
     from .. import ops
     return ops._pdl and os.environ.get("TLLM_PDL", "1") != "0"
