@@ -254,7 +254,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         tile_at(t, tm, tn);
         for (int g = 0; g < p.groups; ++g, ++it) {
           const int s = it % STAGES;
-          if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { *abort_flag = 1; atomicExch(status, ERR_F8_PRODUCER); ok = false; break; }
+          if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { *abort_flag = 1; atomicExch(status, ERR_QP_PRODUCER); ok = false; break; }
           uint8_t* dst = smem + s * L::STAGE_BYTES;
           mbar_expect_tx(&full_bar[s], L::STAGE_BYTES);
           tma_load_2d(dst, &map_a, g * BK, tm * BM, &full_bar[s]);
@@ -285,7 +285,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
           }
           __syncwarp();
         }
-      if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_MMA); }
+      if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_QP_MMA); }
     }
   } else {
     regs_up<REGS_SUMS>();
@@ -349,7 +349,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
           }
         }
       }
-      if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_SUMS); }
+      if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_QP_SUMS); }
       if (!sums_all(ok)) break;
       if (!GATED) {
 #pragma unroll
@@ -490,7 +490,7 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
       for (; i < n_g; ++i) {
         const int s = i % STAGES;
         if (i >= n_pre) {
-          if (!mbar_wait(&empty_bar[s], ((i / STAGES) & 1) ^ 1, abort_flag)) { *abort_flag = 1; atomicExch(status, ERR_F8_PRODUCER); break; }
+          if (!mbar_wait(&empty_bar[s], ((i / STAGES) & 1) ^ 1, abort_flag)) { *abort_flag = 1; atomicExch(status, ERR_QP_PRODUCER); break; }
           load_weight(i, policy);
         }
         tma_load_2d(smem + s * L::STAGE_BYTES + L::W_BYTES, &map_a, (g_begin + i) * BK, m0, &full_bar[s]);
@@ -519,7 +519,7 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
       }
       __syncwarp();
     }
-    if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_MMA); }
+    if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_QP_MMA); }
   } else {
     // ---------------- sums: warp w reads tensor-memory lanes [32 (w % 4), +32) of its tile's accumulator, COLS columns of it
     constexpr int COLS = BN / HALVES;
@@ -587,7 +587,7 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         if (lane == 0) mbar_arrive(&acc_empty[buf]);
       }
     }
-    if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_SUMS); }
+    if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_QP_SUMS); }
     int owner = col0 % f.slices, place = col0 / f.slices;
 #pragma unroll
     for (int j = 0; j < COLS; ++j) {
@@ -606,7 +606,7 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
 
   if (SLICED) cluster_arrive();        // this CTA has sent what it had to
   const bool here = !SLICED || own_tokens == 0 || mbar_wait(sums_bar, 0, abort_flag);
-  if (!here && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_F8_SUMS); }
+  if (!here && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_QP_SUMS); }
   for (int i = here ? warp : own_tokens; i < own_tokens; i += WARPS) {
     const int m = m0 + rank + i * f.slices, n = tile * 128 + 4 * lane;
     float4 part[TILES][8];
@@ -762,7 +762,8 @@ static int most_clusters(int slices) {
   int n = held[dev][slices].load(std::memory_order_relaxed);
   if (n > 0) return n - 1;
   auto kern = linear_fp8_few_kernel<BN, STAGES, GATED, HALVES, true>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL) != cudaSuccess) return 0;
+  static PerDeviceLimit limit;
+  if (reserve_smem(limit, L::TOTAL, kern) != cudaSuccess) return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(1, 1, slices);
   cfg.blockDim = dim3(L::THREADS);
@@ -831,22 +832,33 @@ extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
   cudaStream_t s = (cudaStream_t)stream;
   const int w_rows = gated ? 256 * ((n + 127) / 128) : n;
   const long long w_tiles = (n + 127) / 128;
-  // Few rows of A, or so few tiles that K has to be cut to fill the SMs: the weight's 128 rows as the large side (few).  Otherwise tiles
-  // of 128 x 256 when they fill half the SMs, else of 128 x 128.  us, few / 128 x 128 / 128 x 256 (columns x values of K):
-  //   2,560 x 2,048 of 128 rows 7.5 / 9.6 / 13.4, 256 8.9 / 9.8 / 13.4, 512 13.0 / 10.1 / 13.7, 1,024 25 / 17.4 / 14.3
-  //   4,096 x 4,096 of 256 13.1 / 14.5 / 20, 512 20 / 14.8 / 20, 1,024 40 / 27 / 21
-  //   4,096 x 14,336 of 128 20 / 40 / 53, 256 32 / 40 / 53, 512 58 / 40 / 53, 1,024 116 / 78 / 59
-  // gated, few / 128 x 256: 5,632 x 2,048 of 64 rows 11.0 / 14.8, 128 14.7 / 15.4, 256 29 / 16; 14,336 x 4,096 of 64 24.8 / 27.9, 128 45 / 28
+  // Few rows of A, or so few tiles that K has to be cut to fill the SMs: the weight's 128 rows as the large side (few), with as many rows
+  // of A beside them as keep what the CTAs fetch of the weight within 36 MB and them at once on the SMs: small tiles have the shorter
+  // way from the first product to the last store.  Otherwise tiles of 128 x 256 when they fill half the SMs, else of 128 x 128.
+  // us, few with 16 / 32 / 64 / 128 rows (columns x values of K):
+  //   2,560 x 2,048 of 32 rows 4.4 / 5.0 / 5.9 / 6.4, 64 5.4 / 5.4 / 6.2 / 6.3, 128 - / 6.8 / 7.0 / 7.1, 256 - / 9.0 / 9.4 / 8.9
+  //   4,096 x 4,096 of 64 8.6 / 7.8 / 8.7 / 8.7, 130 - / 14.2 / 14.2 / 12.9; 4,096 x 14,336 of 64 19.7 / 16.1 / 14.9 / 17.2
+  //   300 x 300 of 300 - / 3.6 / 4.2 / 6.1; 1,000 x 1,000 of 1,000 - / 6.8 / 8.8 / 8.4
+  //   gated 5,632 x 2,048 of 32 9.2 / 8.3 / 9.3, 64 11.1 / 14.6 / 10.7; 300 x 300 of 300 4.4 / 5.8 / 6.6
+  // few / 128 x 128 / 128 x 256:
+  //   2,560 x 2,048 of 128 rows 7.1 / 9.6 / 13.4, 256 8.9 / 9.4 / 13.4, 512 11.2 / 9.8 / 13.7, 1,024 25 / 17.4 / 14.3
+  //   4,096 x 4,096 of 256 13.4 / 14.7 / 20, 512 20 / 14.8 / 20, 1,024 40 / 27 / 21
+  //   4,096 x 14,336 of 128 18.7 / 40 / 53, 256 32 / 40 / 53, 512 58 / 40 / 53, 1,024 116 / 78 / 59
+  // gated, few / 128 x 256: 5,632 x 2,048 of 64 rows 10.7 / 14.9, 128 14.2 / 15.4, 256 29 / 16; 14,336 x 4,096 of 64 23.7 / 26.4, 128 45 / 28
+  auto fits = [&](int rows, int resident) {
+    const long long parts = (m + rows - 1) / rows;
+    return m <= rows || (parts * w_rows * k <= 36000000 && parts * w_tiles <= 148 * resident);
+  };
 #define TLLM_FEW(BN, STAGES, WHOLE, GATED, HALVES) return launch_few_rows<BN, STAGES, WHOLE, GATED, HALVES>(p, a, lda, w, ldw, w_rows, k, status, s)
 #define TLLM_TILES(BN, STAGES, GATED) return launch_tiles<BN, STAGES, GATED>(p, a, lda, w, ldw, w_rows, k, status, s)
   if (gated) {
-    if (m <= 16) TLLM_FEW(16, 2, 3, true, 1);
-    if (m <= 32) TLLM_FEW(32, 4, 3, true, 1);
+    if (fits(16, 2)) TLLM_FEW(16, 2, 3, true, 1);
+    if (fits(32, 1)) TLLM_FEW(32, 4, 5, true, 1);
     if (m <= 64 || ((m + 63) / 64) * w_tiles <= 148) TLLM_FEW(64, 3, 5, true, 2);
     TLLM_TILES(256, 4, true);
   }
-  if (m <= 16) TLLM_FEW(16, 5, 6, false, 1);
-  if (m <= 32) TLLM_FEW(32, 4, 5, false, 1);
+  if (fits(16, 2)) TLLM_FEW(16, 5, 6, false, 1);
+  if (fits(32, 2)) TLLM_FEW(32, 4, 5, false, 1);
   if (m <= 64) TLLM_FEW(64, 3, 4, false, 2);
   if (((m + 127) / 128) * w_tiles <= 74) TLLM_FEW(128, 4, 6, false, 4);
   if (((m + 127) / 128) * (long long)((n + 255) / 256) >= 74) TLLM_TILES(256, 4, false);
