@@ -70,7 +70,11 @@ __device__ __forceinline__ float min_nan(float x, float y) { float r; asm("min.N
 __device__ __forceinline__ float gate_f(float g, float u, const Gate& q) {
   g = min_nan(max_nan(g, q.g_low), q.g_high);
   u = min_nan(max_nan(u, -q.u_most), q.u_most);
-  return __fdividef(g, 1.f + expf(-g * fmaf(q.b * g, g, q.a))) * fmaf(q.c, u, q.d);
+  // the quotient to half a unit: an approximate reciprocal and one step with the exact remainder (exp(88) is finite and far beyond what
+  // leaves anything of g); where the result is rounded to 8 bits, every unit moves values across borders
+  const float d = 1.f + expf(min_nan(-g * fmaf(q.b * g, g, q.a), 88.f));
+  const float r = __fdividef(1.f, d), y = g * r;
+  return fmaf(fmaf(-y, d, g), r, y) * fmaf(q.c, u, q.d);
 }
 
 // e4m3 x e4m3 -> float32, M = m, N = n, both operands K-major (bits 7-9 and 10-12: 0 is e4m3)
