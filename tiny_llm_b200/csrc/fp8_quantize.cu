@@ -129,8 +129,8 @@ quantize_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict
   if (lane < GROUPS && g0 + lane < groups) scales[row * lds + g0 + lane] = (uint8_t)mine;
 }
 
-// A CTA per row: y = (w x) / sqrt(mean(x^2) + eps) in 32 bits.  Warp i of W takes the groups i, i + W, ...: PER of them, which stay
-// in registers between the sum and the rounding (PER = 0: any number, read twice).  FULL: the row is whole groups, on 16 bytes.
+// A CTA per row: y = (w x) / sqrt(mean(x^2) + eps) in 32 bits.  A warp takes PER neighbouring groups, which stay in registers between
+// the sum and the rounding, and stores their scales at once (PER = 0: every group that is left, read twice).  FULL: the row is whole groups, on 16 bytes.
 template <int PER, bool FULL>
 __global__ void rms_norm_rows_kernel(const float* __restrict__ x, const float* __restrict__ w, uint8_t* __restrict__ out, long long ldo,
                                      uint8_t* __restrict__ scales, long long lds, const int* __restrict__ gather, int width, int groups,
@@ -152,11 +152,12 @@ __global__ void rms_norm_rows_kernel(const float* __restrict__ x, const float* _
   // the gains come in batches, the first while the row's sum is under way
   constexpr int BATCH = PER >= 4 ? 4 : PER > 0 ? PER : 1;
   float v[PER > 0 ? PER : 1][4], gain[BATCH][4], sum = 0.f;
+  const int g0 = warp * PER;
   if (PER > 0) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) load(src, warp + i * warps, v[i]);
+    for (int i = 0; i < PER; ++i) load(src, g0 + i, v[i]);
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i) load(w, warp + i * warps, gain[i]);
+    for (int i = 0; i < BATCH; ++i) load(w, g0 + i, gain[i]);
 #pragma unroll
     for (int i = 0; i < PER; ++i) sum += v[i][0] * v[i][0] + v[i][1] * v[i][1] + v[i][2] * v[i][2] + v[i][3] * v[i][3];
   } else {
@@ -173,25 +174,31 @@ __global__ void rms_norm_rows_kernel(const float* __restrict__ x, const float* _
   auto leave = [&](int g, float* y, const float* f) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = (f[e] * y[e]) * inv;
-    const uint32_t byte = leave_group(y, dst, g * FP8_GROUP + 4 * lane, FULL ? INT_MAX : width);
-    if (lane == 0) scales[(size_t)blockIdx.x * lds + g] = (uint8_t)byte;
+    return leave_group(y, dst, g * FP8_GROUP + 4 * lane, FULL ? INT_MAX : width);
   };
+  uint8_t* row_scales = scales + (size_t)blockIdx.x * lds;
   if (PER > 0) {
+    uint32_t mine = 0u;      // lane i keeps the byte of the warp's group i
 #pragma unroll
     for (int h = 0; h < PER; h += BATCH) {
       if (h > 0) {
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) load(w, warp + (h + i) * warps, gain[i]);
+        for (int i = 0; i < BATCH; ++i) load(w, g0 + h + i, gain[i]);
       }
 #pragma unroll
       for (int i = 0; i < BATCH; ++i)
-        if (warp + (h + i) * warps < groups) leave(warp + (h + i) * warps, v[h + i], gain[i]);
+        if (g0 + h + i < groups) {
+          const uint32_t byte = leave(g0 + h + i, v[h + i], gain[i]);
+          mine = lane == h + i ? byte : mine;
+        }
     }
+    if (lane < PER && g0 + lane < groups) row_scales[g0 + lane] = (uint8_t)mine;
   } else {
     for (int g = warp; g < groups; g += warps) {
       load(src, g, v[0]);
       load(w, g, gain[0]);
-      leave(g, v[0], gain[0]);
+      const uint32_t byte = leave(g, v[0], gain[0]);
+      if (lane == 0) row_scales[g] = (uint8_t)byte;
     }
   }
 }
