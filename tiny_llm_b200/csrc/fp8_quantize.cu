@@ -290,13 +290,18 @@ extern "C" int tllm_quantize_fp8(const QuantizeCall* c) {
   const unsigned blocks = ((unsigned)rows * runs + ROWS_THREADS / 32 - 1) / (ROWS_THREADS / 32);
   const int vec = (uintptr_t)x % 16 == 0 && ldx % (dtype == TLLM_F32 ? 4 : 8) == 0;
   cudaStream_t s = (cudaStream_t)stream;
-  auto launch = [&](auto zero, auto kern) -> int {
-    using T = decltype(zero);
-    TLLM_LAUNCH("quantize_fp8", kern, blocks, ROWS_THREADS, 0, s, (const T*)x, ldx, (uint8_t*)out, ldo, (uint8_t*)scales, lds, rows, width, groups, runs, vec);
-    return TLLM_OK;
-  };
-  if (dtype == TLLM_F32) return launch(0.f, few ? quantize_rows_kernel<float, Run<float>::SHORT> : quantize_rows_kernel<float, Run<float>::LONG>);
-  return launch(__nv_bfloat16(), few ? quantize_rows_kernel<__nv_bfloat16, Run<__nv_bfloat16>::SHORT> : quantize_rows_kernel<__nv_bfloat16, Run<__nv_bfloat16>::LONG>);
+#define TLLM_ROWS(T, GROUPS)                                                                                                      \
+  TLLM_LAUNCH("quantize_fp8", (quantize_rows_kernel<T, GROUPS>), blocks, ROWS_THREADS, 0, s, (const T*)x, ldx, (uint8_t*)out, ldo, \
+              (uint8_t*)scales, lds, rows, width, groups, runs, vec)
+  if (dtype == TLLM_F32) {
+    if (few) TLLM_ROWS(float, Run<float>::SHORT);
+    else TLLM_ROWS(float, Run<float>::LONG);
+  } else {
+    if (few) TLLM_ROWS(__nv_bfloat16, Run<__nv_bfloat16>::SHORT);
+    else TLLM_ROWS(__nv_bfloat16, Run<__nv_bfloat16>::LONG);
+  }
+#undef TLLM_ROWS
+  return TLLM_OK;
 }
 
 struct RmsNormCall { const float *x, *w; void* out; long long ldo; void* scales; long long lds; const int* rows_idx; int rows, width; float eps; void* stream; };

@@ -839,31 +839,32 @@ extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
   const int w_rows = gated ? 256 * ((n + 127) / 128) : n;
   const long long w_tiles = (n + 127) / 128;
   // Few rows of A, or so few tiles that K has to be cut to fill the SMs: the weight's 128 rows as the large side (few), with as many rows
-  // of A beside them as keep what the CTAs fetch of the weight within 36 MB and them at once on the SMs: small tiles have the shorter
+  // of A beside them as keep what the CTAs fetch of the weight within 36 MB and them at once on the SMs (16 rows: one per SM): small tiles have the shorter
   // way from the first product to the last store.  Otherwise tiles of 128 x 256 when they fill half the SMs, else of 128 x 128.
   // us, few with 16 / 32 / 64 / 128 rows (columns x values of K):
-  //   2,560 x 2,048 of 32 rows 4.4 / 5.0 / 5.9 / 6.4, 64 5.4 / 5.4 / 6.2 / 6.3, 128 - / 6.8 / 7.0 / 7.1, 256 - / 9.0 / 9.4 / 8.9
-  //   4,096 x 4,096 of 64 8.6 / 7.8 / 8.7 / 8.7, 130 - / 14.2 / 14.2 / 12.9; 4,096 x 14,336 of 64 19.7 / 16.1 / 14.9 / 17.2
-  //   300 x 300 of 300 - / 3.6 / 4.2 / 6.1; 1,000 x 1,000 of 1,000 - / 6.8 / 8.8 / 8.4
-  //   gated 5,632 x 2,048 of 32 9.2 / 8.3 / 9.3, 64 11.1 / 14.6 / 10.7; 300 x 300 of 300 4.4 / 5.8 / 6.6
+  //   2,560 x 2,048 of 32 rows 3.8 / 4.7 / 5.6 / 5.8, 64 4.8 / 5.0 / 6.2 / 5.8, 128 6.5 / 6.0 / 6.8 / 6.7, 256 12.2 / 8.6 / 8.6 / 8.4
+  //   4,096 x 4,096 of 64 7.8 / 7.1 / 8.3 / 8.2; 4,096 x 14,336 of 64 18.8 / 15.3 / 13.8 / 16.6
+  //   300 x 300 of 300 3.0 / 3.7 / 4.3 / 6.1; 1,000 x 1,520 of 333 6.3 / 5.8 / 7.1 / 6.7; 1,000 x 1,000 of 1,000 12.1 / 6.8 / 8.0 / 7.8
+  //   gated 5,632 x 2,048 of 32 8.4 / 8.1 / 9.1, 64 11.2 / 10.6 / 10.2; 300 x 300 of 300 4.5 / 5.4 / 6.8
   // few / 128 x 128 / 128 x 256:
   //   2,560 x 2,048 of 128 rows 7.1 / 9.6 / 13.4, 256 8.9 / 9.4 / 13.4, 512 11.2 / 9.8 / 13.7, 1,024 25 / 17.4 / 14.3
   //   4,096 x 4,096 of 256 13.4 / 14.7 / 20, 512 20 / 14.8 / 20, 1,024 40 / 27 / 21
   //   4,096 x 14,336 of 128 18.7 / 40 / 53, 256 32 / 40 / 53, 512 58 / 40 / 53, 1,024 116 / 78 / 59
   // gated, few / 128 x 256: 5,632 x 2,048 of 64 rows 10.7 / 14.9, 128 14.2 / 15.4, 256 29 / 16; 14,336 x 4,096 of 64 23.7 / 26.4, 128 45 / 28
-  auto fits = [&](int rows, int resident) {
-    const long long parts = (m + rows - 1) / rows;
-    return m <= rows || (parts * w_rows * k <= 36000000 && parts * w_tiles <= 148 * resident);
+  const long long w_values = (long long)w_rows * k;
+  auto fits = [&p, w_tiles, w_values](int rows, int resident) {
+    const long long parts = (p.m + rows - 1) / rows;
+    return p.m <= rows || (parts * w_values <= 36000000 && parts * w_tiles <= 148 * resident);
   };
 #define TLLM_FEW(BN, STAGES, WHOLE, GATED, HALVES) return launch_few_rows<BN, STAGES, WHOLE, GATED, HALVES>(p, a, lda, w, ldw, w_rows, k, status, s)
 #define TLLM_TILES(BN, STAGES, GATED) return launch_tiles<BN, STAGES, GATED>(p, a, lda, w, ldw, w_rows, k, status, s)
   if (gated) {
-    if (fits(16, 2)) TLLM_FEW(16, 2, 3, true, 1);
+    if (fits(16, 1)) TLLM_FEW(16, 2, 3, true, 1);
     if (fits(32, 1)) TLLM_FEW(32, 4, 5, true, 1);
     if (m <= 64 || ((m + 63) / 64) * w_tiles <= 148) TLLM_FEW(64, 3, 5, true, 2);
     TLLM_TILES(256, 4, true);
   }
-  if (fits(16, 2)) TLLM_FEW(16, 5, 6, false, 1);
+  if (fits(16, 1)) TLLM_FEW(16, 5, 6, false, 1);
   if (fits(32, 2)) TLLM_FEW(32, 4, 5, false, 1);
   if (m <= 64) TLLM_FEW(64, 3, 4, false, 2);
   if (((m + 127) / 128) * w_tiles <= 74) TLLM_FEW(128, 4, 6, false, 4);
