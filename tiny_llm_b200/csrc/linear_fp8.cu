@@ -413,29 +413,30 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 // the end of the kernel, of 6,100 for one row of 2,560 x 2,048.  Gated: a CTA has the gate tile and the up tile beside it, two
 // accumulators and four warps for each; the 128 columns that a warp stores are one group of the product behind.
 // A tile's columns are dealt to HALVES sets of four summing warps.
-template <int BN, int STAGES, bool GATED, int HALVES, bool SLICED>
+template <int BN, int STAGES, bool GATED, int HALVES, bool SLICED, int SENT = BN + 8>
 struct FewSmem {
   static constexpr int SUM_WARPS = 4 * (GATED ? 2 : 1) * HALVES, THREADS = 64 + 32 * SUM_WARPS;
-  static constexpr int CHUNK = BN >= 64 ? 4 : 8;                      // groups whose scales are laid out in shared memory at a time
+  static constexpr int CHUNK = BN >= 64 || GATED ? 4 : 8;                      // groups whose scales are laid out in shared memory at a time
   static constexpr int TILES = GATED ? 2 : 1, W_BYTES = TILES * 128 * BK, A_BYTES = BN * BK, STAGE_BYTES = W_BYTES + A_BYTES;
   // The sums: [tokens of this CTA][slices][TILES][128 weight rows].  The peers may send theirs while this CTA still works, so they have a
-  // place of their own (whole tokens per CTA: at most 7 more than BN); a CTA without peers leaves them where the stages were.
+  // place of their own, of SENT = tokens per CTA x slices (at most 7 more than BN); a CTA without peers leaves them where the stages were.
   static constexpr int SUMS_OFFSET = SLICED ? STAGES * STAGE_BYTES : 0;
-  static constexpr int SCALE_OFFSET = STAGES * STAGE_BYTES + (SLICED ? (BN + 8) * TILES * 512 : 0);
+  static constexpr int SCALE_OFFSET = STAGES * STAGE_BYTES + (SLICED ? SENT * TILES * 512 : 0);
   static constexpr int BAR_OFFSET = SCALE_OFFSET + TILES * CHUNK * BN * 4;
   static constexpr int TOTAL = BAR_OFFSET + (2 * STAGES + 5) * 8 + 16 + 1024;
-  static_assert(SLICED || TILES * BN * 512 <= STAGES * STAGE_BYTES, "the sums fit where the stages were");
   static constexpr int RESIDENT = TOTAL <= 113 * 1024 && THREADS <= 320 ? 2 : 1;     // CTAs per SM
+  static_assert(!(GATED && BN == 16) || RESIDENT == 2, "two CTAs per SM");
+  static_assert(SLICED || TILES * BN * 512 <= STAGES * STAGE_BYTES, "the sums fit where the stages were");
 };
 
 struct FewArgs {
   int slices, per_slice;       // slices of K (the cluster), groups per slice (the last may have fewer, or none)
 };
 
-template <int BN, int STAGES, bool GATED, int HALVES, bool SLICED>
-__global__ void __launch_bounds__(FewSmem<BN, STAGES, GATED, HALVES, SLICED>::THREADS, FewSmem<BN, STAGES, GATED, HALVES, SLICED>::RESIDENT)
+template <int BN, int STAGES, bool GATED, int HALVES, bool SLICED, int SENT = BN + 8>
+__global__ void __launch_bounds__(FewSmem<BN, STAGES, GATED, HALVES, SLICED, SENT>::THREADS, FewSmem<BN, STAGES, GATED, HALVES, SLICED, SENT>::RESIDENT)
 linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const Fp8Args p, const FewArgs f, int* __restrict__ status) {
-  using L = FewSmem<BN, STAGES, GATED, HALVES, SLICED>;
+  using L = FewSmem<BN, STAGES, GATED, HALVES, SLICED, SENT>;
   constexpr int FEW_CHUNK = L::CHUNK, TILES = L::TILES, FEW_SUM_WARPS = L::SUM_WARPS, WARPS = 2 + FEW_SUM_WARPS;
   constexpr uint32_t ACC_COLS = TILES * BN, TMEM_COLS = 2 * ACC_COLS < 32 ? 32 : 2 * ACC_COLS;
   extern __shared__ uint8_t smem_raw[];
@@ -727,10 +728,10 @@ static int launch_tiles(const Fp8Args& p, const void* a, long long lda, const vo
   return TLLM_OK;
 }
 
-template <int BN, int STAGES, bool GATED, int HALVES, bool SLICED>
+template <int BN, int STAGES, bool GATED, int HALVES, bool SLICED, int SENT = BN + 8>
 static int launch_few(const Fp8Args& p, const FewArgs& f, const void* a, long long lda, const void* w, long long ldw, int w_rows, int k, int* status, cudaStream_t s) {
-  using L = FewSmem<BN, STAGES, GATED, HALVES, SLICED>;
-  auto kern = linear_fp8_few_kernel<BN, STAGES, GATED, HALVES, SLICED>;
+  using L = FewSmem<BN, STAGES, GATED, HALVES, SLICED, SENT>;
+  auto kern = linear_fp8_few_kernel<BN, STAGES, GATED, HALVES, SLICED, SENT>;
   TLLM_RESERVE_SMEM("linear_fp8", L::TOTAL, kern);
   CUtensorMap ma, mw;
   if (!make_map(&mw, w, w_rows, k, ldw, 128) || !make_map(&ma, a, p.m, k, lda, BN)) TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: cannot describe the operands to the copy unit");
@@ -759,15 +760,15 @@ static int launch_few(const Fp8Args& p, const FewArgs& f, const void* a, long lo
 // not divide the group leave some of its SMs idle (with a CTA per SM, 74 of two, 45 of three, 33, 26, 22, 15, 15).  Asked once per kernel,
 // size and device.  The answer counts one CTA per SM for kernels that use tensor memory, of which RESIDENT run (296 CTAs of 128 values of
 // K take 3.0 us, 297 4.4).
-template <int BN, int STAGES, bool GATED, int HALVES>
+template <int BN, int STAGES, bool GATED, int HALVES, int SENT>
 static int most_clusters(int slices) {
-  using L = FewSmem<BN, STAGES, GATED, HALVES, true>;
+  using L = FewSmem<BN, STAGES, GATED, HALVES, true, SENT>;
   static std::atomic<int> held[PerDeviceLimit::DEVICES][9] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= PerDeviceLimit::DEVICES) return 0;
   int n = held[dev][slices].load(std::memory_order_relaxed);
   if (n > 0) return n - 1;
-  auto kern = linear_fp8_few_kernel<BN, STAGES, GATED, HALVES, true>;
+  auto kern = linear_fp8_few_kernel<BN, STAGES, GATED, HALVES, true, SENT>;
   static PerDeviceLimit limit;
   if (reserve_smem(limit, L::TOTAL, kern) != cudaSuccess) return 0;
   cudaLaunchConfig_t cfg = {};
@@ -791,23 +792,31 @@ static int most_clusters(int slices) {
 // two rounds 9.5 us, 5 in one 6.6; 2,560 x 2,048: 8 slices of two groups 4.0, 4 of four 3.8).  Where the slices are long, a few clusters
 // more than run at once cost less than fewer slices (4,096 x 14,336, 32 tiles: 8 slices of 14 groups, 30 clusters at once, 11.0 us, 6 of
 // 19 12.1).
+template <int BN, int STAGES, bool GATED, int HALVES, int SENT>
+static int pick_slices(const Fp8Args& p) {
+  const long long tiles = ((p.n + 127) / 128) * (long long)((p.m + BN - 1) / BN);
+  for (int slices = min(8, p.groups / 4); slices > 1; --slices) {
+    const int most = most_clusters<BN, STAGES, GATED, HALVES, SENT>(slices);
+    if (tiles <= (p.groups >= 12 * slices ? most + most / 15 : most)) return slices;
+  }
+  return 1;
+}
 template <int BN, int STAGES, int STAGES_WHOLE, bool GATED, int HALVES>     // (stages with slices, and without)
 static int launch_few_rows(const Fp8Args& p, const void* a, long long lda, const void* w, long long ldw, int w_rows, int k, int* status, cudaStream_t s) {
-  const long long tiles = ((p.n + 127) / 128) * (long long)((p.m + BN - 1) / BN);
   FewArgs f;
-  f.slices = min(8, p.groups / 4);
-  for (; f.slices > 1; --f.slices) {
-    const int most = most_clusters<BN, STAGES, GATED, HALVES>(f.slices);
-    if (tiles <= (p.groups >= 12 * f.slices ? most + most / 15 : most)) break;
-  }
-  if (f.slices <= 1) {
-    f.slices = 1;
+  f.slices = pick_slices<BN, STAGES, GATED, HALVES, BN + 8>(p);
+  if (f.slices == 1) {
     f.per_slice = p.groups;
-    return launch_few<BN, STAGES_WHOLE, GATED, HALVES, false>(p, f, a, lda, w, ldw, w_rows, k, status, s);
+    return launch_few<BN, STAGES_WHOLE, GATED, HALVES, false, BN + 8>(p, f, a, lda, w, ldw, w_rows, k, status, s);
   }
   f.per_slice = (p.groups + f.slices - 1) / f.slices;
   f.slices = (p.groups + f.per_slice - 1) / f.per_slice;
-  return launch_few<BN, STAGES, GATED, HALVES, true>(p, f, a, lda, w, ldw, w_rows, k, status, s);
+  // Gated rows of a few tokens: the place for the sums is small enough for a third stage beside it, 96 KB of weights in flight per CTA
+  // instead of 64 (8 rows of 5,632 x 2,048 7.2 us -> 5.8, of 2,816 x 2,048 6.0 -> 5.3).
+  if constexpr (GATED && BN == 16) {
+    if ((p.m + f.slices - 1) / f.slices * f.slices <= 9) return launch_few<BN, STAGES + 1, GATED, HALVES, true, 9>(p, f, a, lda, w, ldw, w_rows, k, status, s);
+  }
+  return launch_few<BN, STAGES, GATED, HALVES, true, BN + 8>(p, f, a, lda, w, ldw, w_rows, k, status, s);
 }
 
 }  // namespace tllm
