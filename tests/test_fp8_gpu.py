@@ -192,6 +192,27 @@ def test_gated_products(ops, m, i, k, act, limit):
     ops.check_status()
 
 
+@pytest.mark.parametrize("act,limit", [("silu", 0.0), ("relu", 0.0), ("clamped", 1.5), ("gelu_tanh", 0.0)])
+@pytest.mark.parametrize("m", [3, 100, 2400])
+def test_gates_beyond_32_bits(ops, m, act, limit):
+    """Gate sums of 2^135 (infinite in 32 bits), 2^75, -2^75 and 2^-140 (next to nothing) beside up sums of 128.  The sums are exact, so
+    what is left is the gate's 2^-20 and the rounding to 8 bits of mantissa."""
+    a = rows8(ops, torch.ones(m, 128, device=DEV))
+    w = torch.ones(4, 2, 128, 128, device=DEV)
+    w[2, 0] = -1.0
+    w = weight8(ops, w.view(1024, 128))
+    w[1][0::2] *= torch.tensor([2.0 ** 120, 2.0 ** 68, 2.0 ** 68, 2.0 ** -118], device=DEV)[:, None] * 2.0 ** 8
+    want, _ = fu.gated(*a, *w, 512, act, limit)
+    out = torch.empty(m, 512, dtype=torch.bfloat16, device=DEV)
+    ops.linear_swiglu_fp8(*a, *w, out, act=act, limit=limit)
+    beyond = want.abs() > 2.0 ** 128
+    assert bool(beyond[:, :128].all()) == (act != "clamped") and not bool(beyond[:, 128:].any())
+    assert bool((out[beyond] == math.inf).all())
+    got, want = out.double()[~beyond], want[~beyond]
+    assert bool(((got - want).abs() <= (2.0 ** -8 + 2.0 ** -19) * want.abs() + 2.0 ** -126).all())
+    ops.check_status()
+
+
 # ---------------------------------------------------------------------------------------------- together
 
 

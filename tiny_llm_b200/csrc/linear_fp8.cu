@@ -13,6 +13,7 @@
 // Sizes: any M, N and K; rows of A and W start on 16 bytes.  TMA fills the tails with zeros, the epilogue masks them.  Every wait
 // is bounded: on expiry the kernel records a code in `status`, stops issuing, frees its tensor memory and returns.
 #include <atomic>
+#include <cfloat>
 #include <cmath>
 #include <map>
 #include <mutex>
@@ -72,9 +73,11 @@ __device__ __forceinline__ float gate_f(float g, float u, const Gate& q) {
   u = min_nan(max_nan(u, -q.u_most), q.u_most);
   // the quotient to half a unit: an approximate reciprocal and one step with the exact remainder (exp(88) is finite and far beyond what
   // leaves anything of g); where the result is rounded to 8 bits, every unit moves values across borders
-  const float d = 1.f + expf(min_nan(-g * fmaf(q.b * g, g, q.a), 88.f));
+  // An infinite sum stays infinite: the exponent is taken at 1e15, where every gate has long been its input, and the remainder of an
+  // infinity, a NaN, is dropped.
+  const float h = fminf(g, 1e15f), d = 1.f + expf(min_nan(-h * fmaf(q.b * h, h, q.a), 88.f));
   const float r = __fdividef(1.f, d), y = g * r;
-  return fmaf(fmaf(-y, d, g), r, y) * fmaf(q.c, u, q.d);
+  return fmaf(fmaxf(fmaf(-y, d, g), -FLT_MAX), r, y) * fmaf(q.c, u, q.d);
 }
 
 // e4m3 x e4m3 -> float32, M = m, N = n, both operands K-major (bits 7-9 and 10-12: 0 is e4m3)
