@@ -15,9 +15,6 @@
 #include <atomic>
 #include <cfloat>
 #include <cmath>
-#include <map>
-#include <mutex>
-#include <tuple>
 
 #include "fp8.cuh"
 #include "tc_common.cuh"
@@ -686,26 +683,14 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
 // ---------------------------------------------------------------- host side
 // A 2-D tensor of bytes [rows, k] with row stride ld, tiled in boxes of box_rows x 128.
 static bool make_map(CUtensorMap* map, const void* ptr, int rows, int k, long long ld, int box_rows) {
-  using Key = std::tuple<const void*, int, int, long long, int>;
-  static std::map<Key, CUtensorMap> cache;
-  static std::mutex mu;
-  const Key key(ptr, rows, k, ld, box_rows);
-  std::lock_guard<std::mutex> lock(mu);
-  auto it = cache.find(key);
-  if (it != cache.end()) { *map = it->second; return true; }
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)ld};
   cuuint32_t box[2] = {(cuuint32_t)BK, (cuuint32_t)box_rows};
   cuuint32_t elem[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return false;
-  if (cache.size() > 4096) cache.clear();
-  cache[key] = *map;
-  return true;
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int BN, int STAGES, bool GATED>
@@ -716,11 +701,12 @@ static int launch_tiles(const Fp8Args& p, const void* a, long long lda, const vo
   CUtensorMap ma, mw;
   if (!make_map(&ma, a, p.m, k, lda, BM) || !make_map(&mw, w, w_rows, k, ldw, BN)) TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: cannot describe the operands to the copy unit");
   // the registers that the summing warpgroups ask for are those of the launch, or they would wait for good
-  static int regs = 0;
+  static std::atomic<int> held{0};
+  int regs = held.load(std::memory_order_relaxed);
   if (regs == 0) {
     cudaFuncAttributes fa;
     if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess) TLLM_FAIL(TLLM_ERR_CUDA, "linear_fp8: cannot read the kernel's registers");
-    regs = fa.numRegs;
+    held.store(regs = fa.numRegs, std::memory_order_relaxed);
   }
   TLLM_REQUIRE(regs * THREADS >= 32 * FIRST_SUM_WARP * REGS_OTHERS + 32 * SUM_WARPS * REGS_SUMS, "linear_fp8: built with %d registers, too few for its split", regs);
   const int tiles = ((p.m + BM - 1) / BM) * (GATED ? (p.n + 127) / 128 : (p.n + BN - 1) / BN);
