@@ -369,3 +369,11 @@ def test_threads_on_streams_of_their_own(ops):
     [t.join() for t in threads]
     assert not errors
     assert all(torch.equal(x, y) for p, q in zip(got, want) for x, y in zip(p, q))
+
+
+# ---------------------------------------------------------------------------------------------- ends of the range
+
+
+@pytest.mark.parametrize("m,k", [(2, 25601), (3, 25700), (2, 28672), (2, 28800), (1, 32768), (2, 32769), (300, 25700), (300, 28800), (300, 32768)])
+def test_normed_rows_of_the_widest_ctas(ops, m, k):
+    test_normed_rows(ops, m, k)

@@ -132,9 +132,9 @@ quantize_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict
 // A CTA per row: y = (w x) / sqrt(mean(x^2) + eps) in 32 bits.  A warp takes PER neighbouring groups, which stay in registers between
 // the sum and the rounding, and stores their scales at once (PER = 0: every group that is left, read twice).  FULL: the row is whole groups, on 16 bytes.
 template <int PER, bool FULL>
-__global__ void rms_norm_rows_kernel(const float* __restrict__ x, const float* __restrict__ w, uint8_t* __restrict__ out, long long ldo,
-                                     uint8_t* __restrict__ scales, long long lds, const int* __restrict__ gather, int width, int groups,
-                                     float eps, int vec) {
+__device__ __forceinline__ void rms_norm_row(const float* __restrict__ x, const float* __restrict__ w, uint8_t* __restrict__ out, long long ldo,
+                                             uint8_t* __restrict__ scales, long long lds, const int* __restrict__ gather, int width, int groups,
+                                             float eps, int vec) {
   __shared__ float part[32];
   pdl_trigger();
   pdl_wait();
@@ -201,6 +201,22 @@ __global__ void rms_norm_rows_kernel(const float* __restrict__ x, const float* _
       if (lane == 0) row_scales[g] = (uint8_t)byte;
     }
   }
+}
+template <int PER, bool FULL>
+__global__ void rms_norm_rows_kernel(const float* __restrict__ x, const float* __restrict__ w, uint8_t* __restrict__ out, long long ldo,
+                                     uint8_t* __restrict__ scales, long long lds, const int* __restrict__ gather, int width, int groups,
+                                     float eps, int vec) {
+  rms_norm_row<PER, FULL>(x, w, out, ldo, scales, lds, gather, width, groups, eps, vec);
+}
+// Eight groups per warp want 68 registers (79 where the row is not FULL), of which 28 (25) warps fit an SM.  Rows of more than NORM_WARPS warps
+// run within the 64 that 32 warps may have; for the others that bound changed the order of the loads (2,048 rows of 2,048: 4.9 us,
+// 5.2 with it; of 14,336 30.4 and 31.5).
+constexpr int NORM_WARPS = 24;
+template <bool FULL>
+__global__ void __launch_bounds__(1024)
+rms_norm_wide_rows_kernel(const float* __restrict__ x, const float* __restrict__ w, uint8_t* __restrict__ out, long long ldo,
+                          uint8_t* __restrict__ scales, long long lds, const int* __restrict__ gather, int width, int groups, float eps, int vec) {
+  rms_norm_row<8, FULL>(x, w, out, ldo, scales, lds, gather, width, groups, eps, vec);
 }
 
 constexpr int WEIGHT_THREADS = 512;
@@ -318,7 +334,7 @@ extern "C" int tllm_rms_norm_fp8(const RmsNormCall* c) {
   auto pick = [&](auto whole) {
     constexpr bool F = decltype(whole)::value;
     return warps * per < groups ? rms_norm_rows_kernel<0, F> : per == 1 ? rms_norm_rows_kernel<1, F> : per == 2 ? rms_norm_rows_kernel<2, F>
-           : per == 4 ? rms_norm_rows_kernel<4, F> : rms_norm_rows_kernel<8, F>;
+           : per == 4 ? rms_norm_rows_kernel<4, F> : warps <= NORM_WARPS ? rms_norm_rows_kernel<8, F> : rms_norm_wide_rows_kernel<F>;
   };
   auto kern = full ? pick(std::true_type()) : pick(std::false_type());
   TLLM_LAUNCH("rms_norm_fp8", kern, rows, 32 * warps, 0, (cudaStream_t)stream, x, w, (uint8_t*)out, ldo, (uint8_t*)scales, lds, rows_idx, width, groups, eps, vec);
