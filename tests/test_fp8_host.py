@@ -123,6 +123,21 @@ def test_products_that_do_not_fit(no_device):
             pytest.fail(f"call {i} was not refused")
 
 
+# ---------------------------------------------------------------------------------------------- kernels
+
+
+def test_waits_of_whole_warps_have_one_answer():
+    """A wait that gives up may do so in some lanes of a warp and not in others.  Where all lanes wait, the answer goes through a vote before
+    anything depends on it; the copying lane, which waits alone, is the only one without."""
+    import os
+    from tiny_llm_b200.ops import build
+    with open(os.path.join(build.CSRC, "linear_fp8.cu")) as f:
+        waits = [line.strip() for line in f if "mbar_wait(" in line and not line.lstrip().startswith("//")]
+    assert len(waits) == 7
+    alone = [w for w in waits if "__all_sync(0xffffffffu," not in w]
+    assert len(alone) == 2 and all("mbar_wait(&empty_bar[s]" in w and "ERR_QP_PRODUCER" in w for w in alone)
+
+
 # ---------------------------------------------------------------------------------------------- models
 
 

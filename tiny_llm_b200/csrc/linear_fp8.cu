@@ -612,7 +612,8 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
 
   if (SLICED) cluster_arrive();        // this CTA has sent what it had to
-  const bool here = !SLICED || own_tokens == 0 || mbar_wait(sums_bar, 0, abort_flag);
+  // (one answer for the warp: what follows has steps that all its lanes take together)
+  const bool here = __all_sync(0xffffffffu, !SLICED || own_tokens == 0 || mbar_wait(sums_bar, 0, abort_flag));
   if (!here && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_QP_SUMS); }
   for (int i = here ? warp : own_tokens; i < own_tokens; i += WARPS) {
     const int m = m0 + rank + i * f.slices, n = tile * 128 + 4 * lane;
