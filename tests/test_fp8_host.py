@@ -167,3 +167,41 @@ def test_the_engine_refuses_what_has_no_8_bit_form():
 def test_the_command_line_takes_the_form_of_the_weights():
     from tiny_llm_b200.__main__ import parse_flags
     assert parse_flags(["--weights=fp8"])["weights"] == "fp8" and parse_flags([])["weights"] == ""
+
+
+@pytest.fixture
+def small_model(monkeypatch):
+    """A loaded bfloat16 decoder on the host, whose matrices turn to 8 bits in plain arithmetic."""
+    import fp8_util as fu
+    from conftest import TINY_A
+    from tiny_llm_b200.config import LlamaConfig
+    from tiny_llm_b200.parts import DecoderModel
+
+    def to_fp8(w):
+        q, s = fu.quantize_weight(w)
+        return q.float().to(torch.float8_e4m3fn), s.float()
+    monkeypatch.setattr(ops, "weight_to_fp8", to_fp8)
+    model = DecoderModel(LlamaConfig.from_dict(TINY_A).model_spec())
+    weights = {n: torch.ones([s or 1 for s in w.shape], dtype=torch.bfloat16) for n, w in model.weight_specs().items()}
+    model.load(weights)
+    return model, weights
+
+
+def test_a_model_that_a_runner_uses_is_not_turned(small_model):
+    from tiny_llm_b200.engine.loading import make_runner
+    model, _ = small_model
+    before = [(b.mixer.w_qkv, b.ffn.w_down) for b in model.blocks]
+    make_runner(model, "bfloat16", "cpu", max_tokens=64)
+    with pytest.raises(RuntimeError, match="a runner was built"):
+        model.to_fp8()
+    assert all(b.mixer.w_qkv is x and b.ffn.w_down is y and not b.mixer.fp8 and not b.ffn.fp8 for b, (x, y) in zip(model.blocks, before))
+
+
+def test_a_model_in_8_bits_stays_so(small_model):
+    from tiny_llm_b200.engine.loading import make_runner
+    model, _ = small_model
+    model.to_fp8()
+    held = [b.mixer.w_qkv for b in model.blocks]
+    make_runner(model, "bfloat16", "cpu", max_tokens=64)
+    model.to_fp8()
+    assert all(b.mixer.w_qkv is x and b.mixer.fp8 and b.ffn.fp8 for b, x in zip(model.blocks, held))

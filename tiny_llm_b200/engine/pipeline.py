@@ -65,7 +65,8 @@ class Pipeline:
 
     @classmethod
     def from_model(cls, config, model, **kwargs) -> "Pipeline":
-        """A pipeline around a model that is already loaded on the device (kwargs as the constructor's)."""
+        """A pipeline around a model that is already loaded on the device (kwargs as the constructor's).  `weights`="fp8" turns the
+        model itself, which no other pipeline may use by then; a model in 8 bits stays so whatever `weights` says."""
         return cls((config, model), **kwargs)
 
     @classmethod

@@ -116,6 +116,7 @@ class ModelRunner:
         if not model.loaded:
             raise RuntimeError("the model has no weights yet")
         self.model = model
+        model.has_runner = True
         self.cache = cache
         self.dtype = dtype
         self.device = torch.device(device)

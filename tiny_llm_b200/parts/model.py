@@ -297,6 +297,7 @@ class DecoderModel:
         self.depth_weights = []      # per layer, when the model averages its results over the depth
         self.lm_head = None
         self.loaded = False
+        self.has_runner = False      # a runner was built around the model: its graphs and tapes hold the matrices' addresses
         # a callable(position in the run order, float32 stream [T, H]) called after every layer call: for tests and
         # debugging only (a runner built around a model with a probe must not capture or tape its steps)
         self.probe = None
@@ -361,7 +362,8 @@ class DecoderModel:
     def to_fp8(self) -> None:
         """Turns the matrices of every layer to 8 bits (e4m3 with a scale per block of 128 x 128); from then on their inputs are
         rounded to 8 bits too, with a scale per row and group of 128.  The embedding table, the output matrix, the norms and
-        the cache stay as they are.  For a loaded bfloat16 model whose parts all have an 8-bit form, before a runner is built."""
+        the cache stay as they are.  For a loaded bfloat16 model whose parts all have an 8-bit form, before a runner or a pipeline is built
+        around it (the steps that those keep read the matrices that are given up here); a model that is in 8 bits already stays so."""
         if not self.loaded:
             raise RuntimeError("the model has no weights yet")
         without = [ls.prefix for ls, b in zip(self.spec.layers, self.blocks) if not getattr(b, "has_fp8", bool)()]
@@ -369,6 +371,9 @@ class DecoderModel:
             raise ValueError(f"8-bit weights: layers {without} have parts without an 8-bit form")
         if self.embed.dtype != torch.bfloat16:
             raise ValueError(f"8-bit weights are for the bfloat16 engine, not {self.embed.dtype}")
+        if self.has_runner and not all(x.fp8 for b in self.blocks for x in (b.mixer, b.ffn) if x is not None):
+            raise RuntimeError("8-bit weights: a runner was built around this model, and its graphs read the matrices as they are; "
+                               "turn the model before its first pipeline")
         for b in self.blocks:
             if not getattr(b.mixer, "fp8", False):
                 b.to_fp8()
