@@ -205,3 +205,15 @@ def test_a_model_in_8_bits_stays_so(small_model):
     make_runner(model, "bfloat16", "cpu", max_tokens=64)
     model.to_fp8()
     assert all(b.mixer.w_qkv is x and b.mixer.fp8 and b.ffn.fp8 for b, x in zip(model.blocks, held))
+
+
+def test_a_model_in_8_bits_loads_again(small_model):
+    """New weights are bfloat16 matrices again, whole layers of them, until the model is turned again."""
+    model, weights = small_model
+    model.to_fp8()
+    assert all(isinstance(x, tuple) for b in model.blocks for x in (b.mixer.w_qkv, b.mixer.w_o, b.ffn.w_gate_up, b.ffn.w_down))
+    model.load(weights)
+    assert all(isinstance(x, torch.Tensor) for b in model.blocks for x in (b.mixer.w_qkv, b.mixer.w_o, b.ffn.w_gate_up, b.ffn.w_down))
+    assert not any(b.mixer.fp8 or b.ffn.fp8 for b in model.blocks)
+    model.to_fp8()
+    assert all(isinstance(b.ffn.w_down, tuple) and isinstance(b.mixer.w_o, tuple) for b in model.blocks)

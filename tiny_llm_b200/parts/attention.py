@@ -66,6 +66,7 @@ class GQAttention:
         names = ["q_proj.weight"] if self.shares_cache else ["q_proj.weight", "k_proj.weight", "v_proj.weight"]
         self.w_qkv = torch.cat([weights[prefix + n] for n in names], dim=0).contiguous()
         self.w_o = weights[prefix + "o_proj.weight"]
+        self.fp8 = False
         self.position.prepare(self.w_o.device)
 
     def to_fp8(self) -> None:

@@ -74,6 +74,7 @@ class SwiGLU:
         g, u, d = self.names
         self.w_gate_up = interleave_gate_up(weights[prefix + g], weights[prefix + u], self.block)
         self.w_down = scaled_matrix(weights[prefix + d], self.out_scale)
+        self.fp8 = False
 
     def to_fp8(self) -> None:
         """Turns the loaded matrices to 8 bits.  Gate and up alternate in blocks of 128 rows there, whatever the sizes: the last
