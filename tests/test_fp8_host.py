@@ -217,3 +217,21 @@ def test_a_model_in_8_bits_loads_again(small_model):
     assert not any(b.mixer.fp8 or b.ffn.fp8 for b in model.blocks)
     model.to_fp8()
     assert all(isinstance(b.ffn.w_down, tuple) and isinstance(b.mixer.w_o, tuple) for b in model.blocks)
+
+
+def test_turning_a_model_goes_on_where_it_broke_off(small_model, monkeypatch):
+    model, _ = small_model
+    turn, calls = ops.weight_to_fp8, []
+
+    def breaks(w):
+        calls.append(w)
+        if len(calls) == 4:      # the first layer's down matrix
+            raise MemoryError
+        return turn(w)
+    monkeypatch.setattr(ops, "weight_to_fp8", breaks)
+    with pytest.raises(MemoryError):
+        model.to_fp8()
+    first = model.blocks[0]
+    assert first.mixer.fp8 and not first.ffn.fp8 and isinstance(first.ffn.w_gate_up, torch.Tensor) and isinstance(first.ffn.w_down, torch.Tensor)
+    model.to_fp8()
+    assert all(b.mixer.fp8 and b.ffn.fp8 and isinstance(b.ffn.w_gate_up, tuple) and isinstance(b.ffn.w_down, tuple) for b in model.blocks)

@@ -71,6 +71,8 @@ class GQAttention:
 
     def to_fp8(self) -> None:
         """Turns the loaded matrices to 8 bits; queries, keys, values and the cache stay in the engine's dtype."""
+        if self.fp8:
+            return
         self.w_qkv, self.w_o = ops.weight_to_fp8(self.w_qkv), ops.weight_to_fp8(self.w_o)
         self.fp8 = True
 

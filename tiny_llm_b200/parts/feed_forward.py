@@ -79,10 +79,11 @@ class SwiGLU:
     def to_fp8(self) -> None:
         """Turns the loaded matrices to 8 bits.  Gate and up alternate in blocks of 128 rows there, whatever the sizes: the last
         block of each is filled with zero rows."""
+        if self.fp8:
+            return
         rows, pad = self.w_gate_up.view(-1, 2, self.block, self.hidden_size), -self.intermediate_size % ops.FP8_GROUP
         gate, up = (torch.nn.functional.pad(rows[:, side].reshape(self.intermediate_size, -1), (0, 0, 0, pad)) for side in (0, 1))
-        self.w_gate_up = ops.weight_to_fp8(interleave_gate_up(gate, up, ops.FP8_GROUP))
-        self.w_down = ops.weight_to_fp8(self.w_down)
+        self.w_gate_up, self.w_down = ops.weight_to_fp8(interleave_gate_up(gate, up, ops.FP8_GROUP)), ops.weight_to_fp8(self.w_down)
         self.fp8 = True
 
     def forward(self, ctx, h, resid) -> None:

@@ -375,8 +375,7 @@ class DecoderModel:
             raise RuntimeError("8-bit weights: a runner was built around this model, and its graphs read the matrices as they are; "
                                "turn the model before its first pipeline")
         for b in self.blocks:
-            if not getattr(b.mixer, "fp8", False):
-                b.to_fp8()
+            b.to_fp8()
 
     # ---- one step
     def forward(self, ctx) -> torch.Tensor:
