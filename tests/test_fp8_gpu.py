@@ -377,3 +377,22 @@ def test_threads_on_streams_of_their_own(ops):
 @pytest.mark.parametrize("m,k", [(2, 25601), (3, 25700), (2, 28672), (2, 28800), (1, 32768), (2, 32769), (300, 25700), (300, 28800), (300, 32768)])
 def test_normed_rows_of_the_widest_ctas(ops, m, k):
     test_normed_rows(ops, m, k)
+
+
+@pytest.mark.parametrize("m", [3, 100, 2400])
+def test_relu_of_gates_and_ups_at_the_ends(ops, m):
+    """Gate sums of 2^-100, 2^-110, 2^100 and -2^100 beside up sums of 1.5 * 2^127, 2^127, 2^-100 and 2^127: the sums are exact, the
+    product has one rounding to 32 bits and one to bfloat16, below 2^-126 a multiple of 2^-133."""
+    sums, ups = [2.0 ** -100, 2.0 ** -110, 2.0 ** 100, -2.0 ** 100], [1.5 * 2.0 ** 127, -2.0 ** 127, 2.0 ** -100, 2.0 ** 127]
+    a = rows8(ops, torch.ones(m, 128, device=DEV))
+    w = torch.ones(4, 2, 128, 128, device=DEV)
+    for b in range(4):
+        w[b, 0], w[b, 1] = math.copysign(1.0, sums[b]), math.copysign(1.0, ups[b])
+    w = weight8(ops, w.view(-1, 128))
+    for b in range(4):
+        w[1][2 * b], w[1][2 * b + 1] = abs(sums[b]) * 2.0 ** -7 * 2.0 ** -8, abs(ups[b]) * 2.0 ** -7 * 2.0 ** -8      # (the values are 256, and 256 * 2^-8)
+    want = (torch.tensor(sums, dtype=torch.float64).clamp(min=0) * torch.tensor(ups, dtype=torch.float64)).repeat_interleave(128).to(DEV)
+    out = torch.empty(m, 512, dtype=torch.bfloat16, device=DEV)
+    ops.linear_swiglu_fp8(*a, *w, out, act="relu")
+    assert bool(((out.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -23) * want.abs() + 2.0 ** -133).all())
+    ops.check_status()

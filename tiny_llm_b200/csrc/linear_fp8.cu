@@ -38,16 +38,16 @@ constexpr int BAND = 12;         // row tiles per band of the large products' or
 enum Output { OUT_BF16 = 0, OUT_F32 = 1, OUT_ADD = 2, OUT_FP8 = 3 };
 enum Act { ACT_SILU = 0, ACT_RELU = 1, ACT_CLAMPED = 2, ACT_GELU_TANH = 3 };
 
-// act(g) * u for all four gates without a branch (the code is laid out 64 times per thread): with g and u clamped,
-// g / (1 + exp(-g (a + b g^2))) * (c u + d).  SiLU: a = 1; GELU's tanh form z / 2 (1 + tanh(y)) = z / (1 + exp(-2 y)): a = 2 sqrt(2 / pi),
-// b = 0.044715 a; clamped: a = 1.702, d = 1; ReLU: g from 0 on, a = 0, so that 1 / (1 + 1) meets c = 2.
-struct Gate { float g_low, g_high, u_most, a, b, c, d; };
+// act(g) * u for all four gates without a branch (the code is laid out 32 times per thread): with g and u clamped,
+// g / (1 + exp(-g (a + b g^2) - e)) * (u + d).  SiLU: a = 1; GELU's tanh form z / 2 (1 + tanh(y)) = z / (1 + exp(-2 y)): a = 2 sqrt(2 / pi),
+// b = 0.044715 a; clamped: a = 1.702, d = 1; ReLU: g from 0 on, a = 0, and exp(-e) is 0, so that g is what is left.
+struct Gate { float g_low, g_high, u_most, a, b, d, e; };
 static Gate make_gate(int act, float limit) {
   const float inf = INFINITY;
-  if (act == ACT_RELU) return {0.f, inf, inf, 0.f, 0.f, 2.f, 0.f};
-  if (act == ACT_CLAMPED) return {-inf, limit, limit, 1.702f, 0.f, 1.f, 1.f};
-  if (act == ACT_GELU_TANH) return {-inf, inf, inf, 1.59576912160573081f, 1.59576912160573081f * 0.044715f, 1.f, 0.f};
-  return {-inf, inf, inf, 1.f, 0.f, 1.f, 0.f};
+  if (act == ACT_RELU) return {0.f, inf, inf, 0.f, 0.f, 0.f, 200.f};
+  if (act == ACT_CLAMPED) return {-inf, limit, limit, 1.702f, 0.f, 1.f, 0.f};
+  if (act == ACT_GELU_TANH) return {-inf, inf, inf, 1.59576912160573081f, 1.59576912160573081f * 0.044715f, 0.f, 0.f};
+  return {-inf, inf, inf, 1.f, 0.f, 0.f, 0.f};
 }
 struct Fp8Args {
   const uint8_t* a_scales;     // [m][lda_s] e8m0
@@ -72,9 +72,9 @@ __device__ __forceinline__ float gate_f(float g, float u, const Gate& q) {
   // leaves anything of g); where the result is rounded to 8 bits, every unit moves values across borders
   // An infinite sum stays infinite: the exponent is taken at 1e15, where every gate has long been its input, and the remainder of an
   // infinity, a NaN, is dropped.
-  const float h = fminf(g, 1e15f), d = 1.f + expf(min_nan(-h * fmaf(q.b * h, h, q.a), 88.f));
+  const float h = fminf(g, 1e15f), d = 1.f + expf(min_nan(fmaf(-h, fmaf(q.b * h, h, q.a), -q.e), 88.f));
   const float r = __fdividef(1.f, d), y = g * r;
-  return fmaf(fmaxf(fmaf(-y, d, g), -FLT_MAX), r, y) * fmaf(q.c, u, q.d);
+  return fmaf(fmaxf(fmaf(-y, d, g), -FLT_MAX), r, y) * (u + q.d);
 }
 
 // e4m3 x e4m3 -> float32, M = m, N = n, both operands K-major (bits 7-9 and 10-12: 0 is e4m3)
