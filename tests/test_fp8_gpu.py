@@ -396,3 +396,52 @@ def test_relu_of_gates_and_ups_at_the_ends(ops, m):
     ops.linear_swiglu_fp8(*a, *w, out, act="relu")
     assert bool(((out.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -23) * want.abs() + 2.0 ** -133).all())
     ops.check_status()
+
+
+def exact_gate(g, u, act, limit):
+    """The gates in 64 bits with nothing lost far below zero, and the sigmoid's argument."""
+    if act == "clamped":
+        g, u = g.clamp(max=limit), u.clamp(-limit, limit) + 1
+    t = {"silu": g, "clamped": 1.702 * g, "gelu_tanh": 2 * math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3)}[act]
+    return g * torch.sigmoid(t) * u, t
+
+
+@pytest.mark.parametrize("act,limit", [("silu", 0.0), ("clamped", 2.0 ** 125), ("gelu_tanh", 0.0)])
+@pytest.mark.parametrize("m", [3, 100, 2400])
+def test_gates_far_below_zero(ops, m, act, limit):
+    """Gate sums whose sigmoid is about to leave 32 bits (arguments of -80 to -110, and sums of -2^135, infinite in 32 bits) and small and
+    large positive ones, beside up sums of 2^120 and 1.5 * 2^127.  The argument has three roundings and the constants' (4 * 2^-24 of it), the
+    gate 2^-19 of the value; exp is a multiple of 2^-149 there and off by one, times the gate's input."""
+    at = {"silu": 1.0, "clamped": 1.702, "gelu_tanh": None}[act]
+    args = [80.0, 87.3, 87.4, 87.9, 88.1, 88.6, 89.0, 95.0, 102.0, 110.0]
+    if at is None:      # the sum whose argument this is, by Newton's steps
+        sums = []
+        for t in args:
+            x = 10.0
+            for _ in range(50):
+                x -= (2 * math.sqrt(2 / math.pi) * (x + 0.044715 * x ** 3) - t) / (2 * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * x * x))
+            sums.append(-x)
+    else:
+        sums = [-t / at for t in args]
+    sums += [-2.0 ** 135, 2.0 ** -100, 0.5, 3.0]
+    ups = [2.0 ** 120] * 10 + [2.0, 1.5 * 2.0 ** 127, 1.5 * 2.0 ** 127, 2.0 ** 100]
+    a = rows8(ops, torch.ones(m, 128, device=DEV))
+    w = torch.ones(len(sums), 2, 128, 128, device=DEV)
+    for b, s in enumerate(sums):
+        w[b, 0] = math.copysign(1.0, s)
+    w = weight8(ops, w.view(-1, 128))
+    for b, (s, u) in enumerate(zip(sums, ups)):
+        w[1][2 * b], w[1][2 * b + 1] = abs(s) * 2.0 ** -15, u * 2.0 ** -15      # (the values are 256, and 256 * 2^-8)
+    y = fu.product(*a, *w)[0].view(m, -1, 2, 128)
+    g, u = (y[:, :, side].reshape(m, -1) for side in (0, 1))
+    want, t = exact_gate(g, u, act, limit)
+    out = torch.empty(m, 128 * len(sums), dtype=torch.bfloat16, device=DEV)
+    ops.linear_swiglu_fp8(*a, *w, out, act=act, limit=limit)
+    small = want.abs() < 2.0 ** 127
+    assert bool(small[:, : 12 * 128].all())
+    off = (2.0 ** -8 + 2.0 ** -18 + 4 * 2.0 ** -24 * t.abs().clamp(max=200)) * want.abs() + \
+        (2 * g.abs().clamp(max=200) + 2) * 2.0 ** -149 * (u.clamp(-limit, limit) + 1 if act == "clamped" else u).abs() + 2.0 ** -126
+    got = out.double()
+    assert not bool(torch.isnan(got).any())
+    assert bool(((got - want).abs() <= off)[small].all()) and bool((got[~small].abs() > 2.0 ** 126).all())
+    ops.check_status()

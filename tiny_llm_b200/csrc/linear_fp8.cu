@@ -68,13 +68,15 @@ __device__ __forceinline__ float min_nan(float x, float y) { float r; asm("min.N
 __device__ __forceinline__ float gate_f(float g, float u, const Gate& q) {
   g = min_nan(max_nan(g, q.g_low), q.g_high);
   u = min_nan(max_nan(u, -q.u_most), q.u_most);
-  // the quotient to half a unit: an approximate reciprocal and one step with the exact remainder (exp(88) is finite and far beyond what
-  // leaves anything of g); where the result is rounded to 8 bits, every unit moves values across borders
-  // An infinite sum stays infinite: the exponent is taken at 1e15, where every gate has long been its input, and the remainder of an
-  // infinity, a NaN, is dropped.
-  const float h = fminf(g, 1e15f), d = 1.f + expf(min_nan(fmaf(-h, fmaf(q.b * h, h, q.a), -q.e), 88.f));
-  const float r = __fdividef(1.f, d), y = g * r;
-  return fmaf(fmaxf(fmaf(-y, d, g), -FLT_MAX), r, y) * (u + q.d);
+  // With x = exp(-|argument|), at most 1: g / (1 + x) from zero on and g x / (1 + x) below, so that nothing leaves 32 bits before the
+  // result does.  The quotient to half a unit: an approximate reciprocal of a number from 1 to 2 and one step with the exact remainder;
+  // where the result is rounded to 8 bits, every unit moves values across borders.
+  // An infinite sum stays infinite: the argument is taken at 1e15, where every gate has long been its input, and the remainder of an
+  // infinity, a NaN, is dropped; below zero the gate is 0 there.
+  const float h = min_nan(max_nan(g, -1e15f), 1e15f), x = expf(fmaf(-fabsf(h), fmaf(q.b * h, h, q.a), -q.e));
+  const float n = h < 0.f ? h * x : g, d = 1.f + x;
+  const float r = __fdividef(1.f, d), y = n * r;
+  return fmaf(fmaxf(fmaf(-y, d, n), -FLT_MAX), r, y) * (u + q.d);
 }
 
 // e4m3 x e4m3 -> float32, M = m, N = n, both operands K-major (bits 7-9 and 10-12: 0 is e4m3)
