@@ -445,3 +445,101 @@ def test_gates_far_below_zero(ops, m, act, limit):
     assert not bool(torch.isnan(got).any())
     assert bool(((got - want).abs() <= off)[small].all()) and bool((got[~small].abs() > 2.0 ** 126).all())
     ops.check_status()
+
+
+def far_scales(g, m, n, k):
+    """The first three groups of K.  Rows 0, 4, ...: scale 2^100 on a group whose block has 2^30, with one value of 2^-9 against columns that are
+    zero (the first hundred) or hold 2^-9 (2^-18 * 2^130 is a normal float, 2^130 is none); rows 1, 5, ...: 2^-126 on blocks of
+    1.3 * 2^-12; rows 2, 6, ...: 2^-127 on blocks of 1.7 * 2^-36 (2^-163, and sums of 2^18); the others: nothing far."""
+    a = torch.randn(m, k, generator=g, device=DEV) * 100
+    w = torch.randn(n, k, generator=g, device=DEV) * 100
+    e = torch.full((m, fu.groups(k)), 127, device=DEV)
+    a[:, :128] = 0
+    a[0::4, 5] = 2.0 ** -9
+    w[:, :128] = 0
+    w[100:, :128] = 2.0 ** -9
+    e[0::4, 0], e[1::4, 1], e[2::4, 2] = 227, 1, 0
+    a[1::4, 256:] = 0
+    a[2::4, 128:256] = 0
+    a[1::4, 384:], a[2::4, 384:] = 0, 0
+    rows = (a.clamp(-448, 448).to(torch.float8_e4m3fn), e.to(torch.uint8).view(torch.float8_e8m0fnu))
+    blocks = torch.ones(fu.groups(n), fu.groups(k), device=DEV)
+    blocks[:, :3] = torch.tensor([2.0 ** 30, 1.3 * 2.0 ** -12, 1.7 * 2.0 ** -36], device=DEV)
+    return rows, w.clamp(-448, 448).to(torch.float8_e4m3fn), blocks
+
+
+def in_room(ops, rows, weight):
+    """The same values in rows that start on 16 bytes."""
+    a, w = ops.fp8_rows(*rows[0].shape, DEV), ops.fp8_weight(*weight[0].shape, DEV)
+    for room, t in zip(a + w, rows + weight):
+        room.copy_(t)
+    return a, w
+
+
+@pytest.mark.parametrize("m,n,k", [(4, 130, 300), (5, 700, 1100), (40, 14336, 300), (64, 40000, 300), (128, 4096, 2304), (600, 3000, 300), (700, 8192, 400)])
+def test_scales_whose_product_is_no_normal_float(ops, m, n, k):
+    """The row's scale times the block's may be far outside of 32 bits where the result is not; what is left of a sum below 2^-126 is
+    a multiple of 2^-149."""
+    rows, w, blocks = far_scales(rng(m + n), m, n, k)
+    a, w = in_room(ops, rows, (w, blocks))
+    want, off = fu.product(*a, *w)
+    assert bool((want.abs() < 2.0 ** 120).all())
+    out = torch.empty(m, n, device=DEV)
+    ops.linear_fp8(*a, *w, out)
+    assert bool(((out - want).abs() <= off + 2.0 ** -24 * want.abs() + 3 * 2.0 ** -149).all())
+    stream = randn(rng(m), m, n)
+    acc = stream.clone()
+    ops.linear_fp8(*a, *w, acc, accumulate=True)
+    assert bool(((acc - (stream + want)).abs() <= off + 2.0 ** -24 * ((stream + want).abs() + want.abs() + off)).all())
+    ops.check_status()
+
+
+@pytest.mark.parametrize("m,n,k", [(4, 530, 300), (5, 700, 1100), (600, 3000, 300), (700, 8192, 400)])
+def test_block_scales_of_zero_below_zero_and_nan(ops, m, n, k):
+    """The first block of columns has scales of 0 (a product of 0, and of -0), the second below zero, the third a NaN."""
+    g = rng(m + n)
+    a, w = rows8(ops, randn(g, m, k)), weight8(ops, randn(g, n, k))
+    w[1][0], w[1][1], w[1][2, 1] = 0.0, -w[1][1], math.nan
+    w[1][0, 1] = -0.0
+    out, stream = torch.empty(m, n, device=DEV), randn(g, m, n)
+    acc = stream.clone()
+    ops.linear_fp8(*a, *w, out)
+    ops.linear_fp8(*a, *w, acc, accumulate=True)
+    want, off = fu.product(*a, *w)
+    assert bool((out[:, :128] == 0).all()) and bool((acc[:, :128] == stream[:, :128]).all())
+    assert bool(torch.isnan(out[:, 256:384]).all()) and bool(torch.isnan(acc[:, 256:384]).all())
+    keep = torch.arange(n, device=DEV) // 128 != 2
+    assert bool(((out - want).abs() <= off + 2.0 ** -24 * want.abs())[:, keep].all())
+    assert bool(((acc - (stream + want)).abs() <= off + 2.0 ** -24 * ((stream + want).abs() + want.abs() + off))[:, keep].all())
+    ops.check_status()
+
+
+@pytest.mark.parametrize("m,i", [(4, 130), (40, 6400), (64, 14336), (700, 2500)])
+def test_gated_scales_whose_product_is_no_normal_float(ops, m, i):
+    """Rows 0, 2, ...: a group with 2^100 on blocks of 2^30 that hold zeros.  Rows 1, 3, ...: 2^-126 on gate blocks of 1.3 * 2^-24
+    (sums of about 2^-133) and up blocks of 2^120.  Gate sums come out as
+    multiples of 2^-149, results as multiples of 2^-133."""
+    g, k = rng(m + i), 300
+    x = torch.randn(m, k, generator=g, device=DEV) * 100
+    e = torch.full((m, 3), 127, device=DEV)
+    x[:, 256:] = 0
+    x[1::2, :128] = 0
+    e[0::2, 0], e[1::2, 1] = 227, 1
+    b = fu.groups(i)
+    w = torch.randn(256 * b, k, generator=g, device=DEV) * 100
+    w[:, :128] = 0
+    blocks = torch.ones(2 * b, 3, device=DEV)
+    blocks[:, 0] = 2.0 ** 30
+    blocks[0::2, 1], blocks[1::2, 1] = 1.3 * 2.0 ** -24, 2.0 ** 120
+    x[0::2, 128:256] *= 2.0 ** -14
+    a, w = in_room(ops, (x.clamp(-448, 448).to(torch.float8_e4m3fn), e.to(torch.uint8).view(torch.float8_e8m0fnu)),
+                   (w.clamp(-448, 448).to(torch.float8_e4m3fn), blocks))
+    want, off = fu.gated(*a, *w, i, "silu")
+    up = fu.product(*a, *w)[0].view(m, -1, 2, 128)[:, :, 1].reshape(m, -1)[:, :i]
+    beyond = want.abs() > 2.0 ** 127
+    assert not bool(beyond[1::2].any())
+    out = torch.empty(m, i, dtype=torch.bfloat16, device=DEV)
+    ops.linear_swiglu_fp8(*a, *w, out)
+    assert not bool(torch.isnan(out).any())
+    assert bool(((out.double() - want).abs() <= off + 2.0 ** -8 * (want.abs() + off) + 4 * 2.0 ** -149 * (up.abs() + 1) + 2.0 ** -133)[~beyond].all())
+    ops.check_status()

@@ -15,6 +15,7 @@
 #include <atomic>
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 #include "fp8.cuh"
 #include "tc_common.cuh"
@@ -50,12 +51,13 @@ static Gate make_gate(int act, float limit) {
   return {-inf, inf, inf, 1.f, 0.f, 0.f, 0.f};
 }
 struct Fp8Args {
+  const uint8_t *a, *w;        // e4m3 rows, for far_sum (the products read them through the copy unit)
   const uint8_t* a_scales;     // [m][lda_s] e8m0
   const float* w_scales;       // [ceil(n / 128)][groups]
   void* out;
   uint8_t* out_scales;         // OUT_FP8: [m][ldo_s] e8m0
-  long long lda_s, ldo, ldo_s;
-  int m, n, groups;            // n: columns of `out` (gated: half the weight's rows, without the ones that fill the last block)
+  long long lda, ldw, lda_s, ldo, ldo_s;
+  int m, n, k, w_rows, groups;            // n: columns of `out` (gated: half the weight's rows, without the ones that fill the last block)
   int mode;
   int vec_out;                 // rows of `out` start on 16 bytes
   int vec_scales;              // rows of a_scales start on 4 bytes
@@ -77,6 +79,31 @@ __device__ __forceinline__ float gate_f(float g, float u, const Gate& q) {
   const float n = h < 0.f ? h * x : g, d = 1.f + x;
   const float r = __fdividef(1.f, d), y = n * r;
   return fmaf(fmaxf(fmaf(-y, d, n), -FLT_MAX), r, y) * (u + q.d);
+}
+
+// A group's sum meets the product of two scales, which may lie anywhere in 32 bits: the product may leave them although the result does not
+// (2^100 * 2^40 beside a sum of 0 or 2^-18), or keep few bits below 2^-126.  The kernels note such products, and the elements they belong to are
+// summed once more, one by one and in 64 bits.  The scales of a model's rows and weights lie within a few powers of ten, so this is for
+// being right and not for speed: a row of 14,336 values takes milliseconds, of some millions longer than the other warps wait, which the
+// status word then says.  The way of all others pays an instruction or two per product for it (1 x 2,560 x 2,048 3.08 us -> 3.13, gated
+// 8 x 5,632 x 2,048 5.74 -> 5.82, many rows nothing).  Two factors in place of the product, applied one after the other, cost every call 2 to 7 %.
+__device__ __forceinline__ uint32_t far_key(float s) { return 2u * __float_as_uint(s) - 0x01000000u; }      // FAR or more unless s is a normal number
+constexpr uint32_t FAR = 0xFE000000u;
+// (zeros, infinities and NaN among the scales themselves give what they give)
+__device__ __forceinline__ bool is_far(uint32_t byte, float w) { return far_key(fp8_scale(byte) * w) >= FAR && byte != 255u && w != 0.f && isfinite(w); }
+__device__ __forceinline__ float far_sum(const Fp8Args& p, int m, int w_row) {
+  const uint8_t *a = p.a + m * p.lda, *w = p.w + w_row * p.ldw, *sa = p.a_scales + m * p.lda_s;
+  const float* sw = p.w_scales + (long long)(w_row / 128) * p.groups;
+  auto value = [](uint8_t v) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3))); };
+  double sum = 0.;
+  for (int g = 0; g < p.groups; ++g) {
+    double part = 0.;
+    const int end = min(p.k, (g + 1) * BK);
+#pragma unroll 1
+    for (int k = g * BK; k < end; ++k) part += value(a[k]) * value(w[k]);       // (a product of two has 8 bits)
+    sum += part * fp8_scale(sa[g]) * sw[g];
+  }
+  return (float)sum;
 }
 
 // e4m3 x e4m3 -> float32, M = m, N = n, both operands K-major (bits 7-9 and 10-12: 0 is e4m3)
@@ -210,7 +237,7 @@ __device__ __forceinline__ void store_columns(const Fp8Args& p, float* staging, 
 
 template <int BN, int STAGES, bool GATED>
 __global__ void __launch_bounds__(THREADS, 1)
-linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const Fp8Args p, int* __restrict__ status) {
+linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Fp8Args p, int* __restrict__ status) {
   static_assert(!GATED || BN == 256, "a gated tile is one group of gate columns and one of up columns");
   using L = Smem<BN, STAGES>;
   constexpr int ACCS = L::ACCS;
@@ -329,10 +356,12 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
       uint32_t quad_now = 0u, quad_next = four_scales(0);
       float w0 = sw[0], w1 = GATED ? sw[p.groups] : 0.f;
+      uint32_t farthest = 0u;
       for (int g = 0; g < p.groups; ++g, ++it) {
         const int buf = it % ACCS;
         if ((g & 3) == 0) { quad_now = quad_next; quad_next = four_scales(g + 4); }
         const float a = fp8_scale((quad_now >> (8 * (g & 3))) & 255u), s0 = a * w0, s1 = a * w1;
+        farthest = max(farthest, GATED ? max(far_key(s0), far_key(s1)) : far_key(s0));
         if (g + 1 < p.groups) { w0 = sw[g + 1]; if (GATED) w1 = sw[p.groups + g + 1]; }
         ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (it / ACCS) & 1, abort_flag));
         if (!ok) break;
@@ -359,6 +388,22 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       }
       if (!ok && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_QP_SUMS); }
       if (!sums_all(ok)) break;
+      if (__builtin_expect(__any_sync(0xffffffffu, farthest >= FAR), 0)) {
+        bool far = false;
+        if (farthest >= FAR && m < p.m)
+          for (int g = 0; g < p.groups; ++g) far = far || is_far(sa[g], sw[g]) || (GATED && is_far(sa[g], sw[p.groups + g]));
+        if (far) {
+          float again[COLS];
+#pragma unroll 1
+          for (int j = 0; j < COLS; ++j) {
+            const int w_row = tile_n * BN + column(j / 32) + j % 32;
+            again[j] = w_row < p.w_rows ? far_sum(p, m, w_row) : 0.f;
+          }
+#pragma unroll
+          for (int j = 0; j < COLS; ++j) acc[j] = again[j];
+        }
+        __syncwarp();
+      }
       if (!GATED) {
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) store_columns(p, staging, m - lane, tile_n * BN + column(c), acc + 32 * c, p.mode);
@@ -437,7 +482,7 @@ struct FewArgs {
 
 template <int BN, int STAGES, bool GATED, int HALVES, bool SLICED, int SENT = BN + 8>
 __global__ void __launch_bounds__(FewSmem<BN, STAGES, GATED, HALVES, SLICED, SENT>::THREADS, FewSmem<BN, STAGES, GATED, HALVES, SLICED, SENT>::RESIDENT)
-linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const Fp8Args p, const FewArgs f, int* __restrict__ status) {
+linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ Fp8Args p, const FewArgs f, int* __restrict__ status) {
   using L = FewSmem<BN, STAGES, GATED, HALVES, SLICED, SENT>;
   constexpr int FEW_CHUNK = L::CHUNK, TILES = L::TILES, FEW_SUM_WARPS = L::SUM_WARPS, WARPS = 2 + FEW_SUM_WARPS;
   constexpr uint32_t ACC_COLS = TILES * BN, TMEM_COLS = 2 * ACC_COLS < 32 ? 32 : 2 * ACC_COLS;
@@ -545,9 +590,12 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
       for (int q = 0; q < FETCH; ++q) {
         const int e = thread + q * 32 * FEW_SUM_WARPS, g = e % FEW_CHUNK, j = e / FEW_CHUNK;
         const bool there = j < BN && i0 + g < n_g && m0 + j < p.m;
-        const float a = there ? fp8_scale(p.a_scales[(long long)(m0 + j) * p.lda_s + g_begin + i0 + g]) : 0.f;
+        const float a = there ? fp8_scale(p.a_scales[(long long)(m0 + j) * p.lda_s + g_begin + i0 + g]) : 1.f;
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) fetched[q][t] = there ? a * p.w_scales[(long long)(tile * TILES + t) * p.groups + g_begin + i0 + g] : 0.f;
+        for (int t = 0; t < TILES; ++t) {
+          const float s = there ? a * p.w_scales[(long long)(tile * TILES + t) * p.groups + g_begin + i0 + g] : 1.f;
+          fetched[q][t] = far_key(s) >= FAR ? __uint_as_float(0x7FC00000u) : s;      // (the token's owner sees the NaN)
+        }
       }
     };
     fetch(0);
@@ -617,7 +665,10 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   // (one answer for the warp: what follows has steps that all its lanes take together)
   const bool here = __all_sync(0xffffffffu, !SLICED || own_tokens == 0 || mbar_wait(sums_bar, 0, abort_flag));
   if (!here && lane == 0) { *abort_flag = 1; atomicExch(status, ERR_QP_SUMS); }
-  for (int i = here ? warp : own_tokens; i < own_tokens; i += WARPS) {
+  // Token i of this CTA.  A sum is NaN by scales whose product is no normal number, or by a row's own (or a weight's): such tokens come a second
+  // time, with those sums made one by one (a row with a scale that is NaN stays NaN).  Returns whether the lane has met a NaN.
+  auto leave = [&](int i, auto is_far) -> bool {
+    constexpr bool FAR_SUMS = decltype(is_far)::value;
     const int m = m0 + rank + i * f.slices, n = tile * 128 + 4 * lane;
     float4 part[TILES][8];
 #pragma unroll
@@ -632,6 +683,24 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
 #pragma unroll
       for (int z = 0; z < 8; ++z)
         if (SLICED ? z < f.slices : z == 0) { sum[t][0] += part[t][z].x; sum[t][1] += part[t][z].y; sum[t][2] += part[t][z].z; sum[t][3] += part[t][z].w; }
+    }
+    bool nan = (FAR_SUMS || !GATED) && isnan((sum[0][0] + sum[0][1]) + (sum[0][2] + sum[0][3]));
+    if constexpr (FAR_SUMS) {
+      if (GATED) nan = nan || isnan((sum[TILES - 1][0] + sum[TILES - 1][1]) + (sum[TILES - 1][2] + sum[TILES - 1][3]));
+      if (!__any_sync(0xffffffffu, nan)) return false;
+      bool nan_row = false;
+      for (int g = 0; g < p.groups; ++g) nan_row = nan_row || p.a_scales[m * p.lda_s + g] == 255;
+      if (nan && !nan_row) {
+        float again[4 * TILES];
+#pragma unroll 1
+        for (int j = 0; j < 4 * TILES; ++j) {
+          const int w_row = (tile * TILES + j / 4) * 128 + 4 * lane + j % 4;
+          again[j] = w_row < p.w_rows ? far_sum(p, m, w_row) : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4 * TILES; ++j) sum[j / 4][j % 4] = again[j];
+      }
+      __syncwarp();
     }
     if (GATED) {
 #pragma unroll
@@ -662,7 +731,7 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         for (int e = 0; e < 4; ++e)
           if (n + e < p.n) dst[e] = __float2bfloat16_rn(sum[0][e]);
       }
-    } else {
+    } else if (p.mode != OUT_ADD || nan == FAR_SUMS) {      // (nothing is added twice)
       float* dst = reinterpret_cast<float*>(p.out) + (size_t)m * p.ldo + n;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -675,7 +744,13 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
           if (n + e < p.n) dst[e] = sum[0][e];
       }
     }
-  }
+    if (GATED) nan = isnan((sum[0][0] + sum[0][1]) + (sum[0][2] + sum[0][3]));      // (of either side)
+    return nan;
+  };
+  bool met = false;
+  for (int i = here ? warp : own_tokens; i < own_tokens; i += WARPS) met = leave(i, std::false_type()) || met;
+  if (__builtin_expect(__any_sync(0xffffffffu, met), 0))
+    for (int i = warp; i < own_tokens; i += WARPS) leave(i, std::true_type());
   // Everybody has sent (whoever has its sums knows that already).  A CTA that gave up waiting for them stays until they have landed.
   if (SLICED) {
     cluster_wait();
@@ -828,6 +903,7 @@ extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
   TLLM_REQUIRE(gated ? (mode == OUT_BF16 || mode == OUT_FP8) : (mode >= OUT_BF16 && mode <= OUT_ADD), "linear_fp8: output code %d", mode);
   TLLM_REQUIRE(act >= 0 && act <= 3 && (act != ACT_CLAMPED || limit > 0.f), "linear_fp8: activation code %d, limit %g", act, (double)limit);
   Fp8Args p = {};
+  p.a = (const uint8_t*)a; p.w = (const uint8_t*)w; p.lda = lda; p.ldw = ldw; p.k = k;
   p.a_scales = (const uint8_t*)a_scales; p.w_scales = w_scales; p.out = out; p.out_scales = (uint8_t*)out_scales;
   p.lda_s = lda_s; p.ldo = ldo; p.ldo_s = ldo_s;
   p.m = m; p.n = n; p.groups = (k + BK - 1) / BK;
@@ -838,6 +914,7 @@ extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
   TLLM_REQUIRE(mode != OUT_FP8 || p.vec_out, "linear_fp8: rows of 8-bit values start on 16 bytes");
   cudaStream_t s = (cudaStream_t)stream;
   const int w_rows = gated ? 256 * ((n + 127) / 128) : n;
+  p.w_rows = w_rows;
   const long long w_tiles = (n + 127) / 128;
   // Few rows of A, or so few tiles that K has to be cut to fill the SMs: the weight's 128 rows as the large side (few), with as many rows
   // of A beside them as keep what the CTAs fetch of the weight within 36 MB and them at once on the SMs (16 rows: one per SM): small tiles have the shorter
