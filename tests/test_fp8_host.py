@@ -138,6 +138,36 @@ def test_waits_of_whole_warps_have_one_answer():
     assert len(alone) == 2 and all("mbar_wait(&empty_bar[s]" in w and "ERR_QP_PRODUCER" in w for w in alone)
 
 
+def test_threads_that_load_the_extension_at_once_get_one_module(monkeypatch, tmp_path):
+    """In a fresh build folder, with a compiler that takes its time, so that they do meet."""
+    import shutil
+    import threading
+    from tiny_llm_b200.ops import build
+    source = tmp_path / "csrc"
+    source.mkdir()
+    (source / "two_threads.cpp").write_text("""#include <Python.h>
+        static PyModuleDef module = {PyModuleDef_HEAD_INIT, "two_threads", nullptr, -1, nullptr, nullptr, nullptr, nullptr, nullptr};
+        PyMODINIT_FUNC PyInit_two_threads(void) { return PyModule_Create(&module); }""")
+    slow = tmp_path / "slow_compiler"
+    slow.write_text(f"#!/bin/sh\nsleep 1\n{shutil.which('g++')} \"$@\"\nstatus=$?\nsleep 1\nexit $status\n")
+    slow.chmod(0o755)
+    monkeypatch.setattr(build, "CSRC", str(source))
+    monkeypatch.setenv("TLLM_BUILD_DIR", str(tmp_path / "build"))
+    monkeypatch.setenv("CXX", str(slow))
+    modules, errors = [], []
+
+    def load():
+        try:
+            modules.append(build.load_extension("two_threads"))
+        except Exception as e:
+            errors.append(e)
+    threads = [threading.Thread(target=load) for _ in range(3)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors
+    assert len(modules) == 3 and all(m is modules[0] for m in modules) and modules[0].__name__ == "two_threads"
+
+
 # ---------------------------------------------------------------------------------------------- models
 
 

@@ -167,14 +167,21 @@ def compile_extension(name: str, verbose: bool = True) -> str:
     return out
 
 
+_extensions = {}
+
+
 def load_extension(name: str):
-    """The Python module of csrc/<name>.cpp."""
+    """The Python module of csrc/<name>.cpp, one per process: threads that ask at once wait for the one that builds it."""
     import importlib.machinery
     import importlib.util
-    loader = importlib.machinery.ExtensionFileLoader(name, compile_extension(name))
-    module = importlib.util.module_from_spec(importlib.util.spec_from_loader(name, loader))
-    loader.exec_module(module)
-    return module
+    with _lock:
+        module = _extensions.get(name)
+        if module is None:
+            loader = importlib.machinery.ExtensionFileLoader(name, compile_extension(name))
+            module = importlib.util.module_from_spec(importlib.util.spec_from_loader(name, loader))
+            loader.exec_module(module)
+            _extensions[name] = module
+        return module
 
 
 def _pdl_default() -> bool:
