@@ -138,6 +138,27 @@ def test_waits_of_whole_warps_have_one_answer():
     assert len(alone) == 2 and all("mbar_wait(&empty_bar[s]" in w and "ERR_QP_PRODUCER" in w for w in alone)
 
 
+def test_arguments_have_one_layout():
+    """The structs of the entry points are declared once, and the interpreter packs them by what the libraries say."""
+    import ctypes
+    import os
+    import struct
+    from tiny_llm_b200.ops import build
+    declared = {}
+    for name in os.listdir(build.CSRC):
+        if name.startswith(("fp8", "linear_fp8")) and not name.endswith(".so"):
+            with open(os.path.join(build.CSRC, name)) as f:
+                for line in f:
+                    if line.startswith("struct ") and "Call {" in line:
+                        declared.setdefault(line.split()[1], []).append(name)
+    assert declared == {s: ["fp8_calls.h"] for s in ("QuantizeCall", "RmsNormCall", "QuantizeWeightCall", "LinearFp8Call")}
+    sizes = {"tllm_quantize_fp8": (10, 72), "tllm_rms_norm_fp8": (11, 80), "tllm_quantize_weight_fp8": (9, 64), "tllm_linear_fp8": (20, 136)}
+    for name, (fields, size) in sizes.items():
+        letters = getattr(build.load_library(ops._FP8_ENTRIES[name]), name + "_layout")
+        letters.restype = ctypes.c_char_p
+        assert len(letters()) == fields and struct.calcsize(letters().decode()) == size
+
+
 def test_threads_that_load_the_extension_at_once_get_one_module(monkeypatch, tmp_path):
     """In a fresh build folder, with a compiler that takes its time, so that they do meet."""
     import shutil

@@ -11,15 +11,9 @@
 
 #include <cstdint>
 
-namespace {
+#include "fp8_calls.h"
 
-struct QuantizeCall { const void* x; long long ldx; void* out; long long ldo; void* scales; long long lds; int rows, width, dtype; void* stream; };
-struct RmsNormCall { const float *x, *w; void* out; long long ldo; void* scales; long long lds; const int* rows_idx; int rows, width; float eps; void* stream; };
-struct QuantizeWeightCall { const void* w; long long ldw; void* out; long long ldo; float* scales; int rows, width, dtype; void* stream; };
-struct LinearFp8Call {
-  const void* a; long long lda; const void* a_scales; long long lda_s; const void* w; long long ldw; const float* w_scales; void* out; long long ldo;
-  void* out_scales; long long ldo_s; int m, n, k, mode, gated, act; float limit; int* status; void* stream;
-};
+namespace {
 
 int (*g_quantize)(const QuantizeCall*) = nullptr;
 int (*g_rms_norm)(const RmsNormCall*) = nullptr;
@@ -108,7 +102,7 @@ PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         !matrix(a[4], (int)device, sc) || !values8(out) || !row_scales(sc, out) || x.rows != out.rows || x.cols != out.cols || x.type != at::kFloat ||
         (x.rows > 1 && x.ld != x.cols) || !float_vector(a[1], (int)device, x.cols, &w))
       return false;
-    const RmsNormCall c = {(const float*)x.data, (const float*)w, out.data, out.ld, sc.data, sc.ld, nullptr, (int)x.rows, (int)x.cols,
+    const RmsNormCall c = {x.data, w, out.data, out.ld, sc.data, sc.ld, nullptr, (int)x.rows, (int)x.cols,
                            (float)PyFloat_AS_DOUBLE(a[2]), (void*)stream};
     return launch(g_rms_norm, c);
   });
@@ -122,7 +116,7 @@ PyObject* quantize_weight(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 5 || !number(a[3], device) || !number(a[4], stream) || !matrix(a[0], (int)device, w) || !matrix(a[1], (int)device, out) ||
         !matrix(a[2], (int)device, sc) || !values8(out) || !weight_scales(sc, out) || w.rows != out.rows || w.cols != out.cols || float_code(w.type) < 0)
       return false;
-    const QuantizeWeightCall c = {w.data, w.ld, out.data, out.ld, (float*)sc.data, (int)w.rows, (int)w.cols, float_code(w.type), (void*)stream};
+    const QuantizeWeightCall c = {w.data, w.ld, out.data, out.ld, sc.data, (int)w.rows, (int)w.cols, float_code(w.type), (void*)stream};
     return launch(g_quantize_weight, c);
   });
 }
@@ -133,7 +127,7 @@ bool operands(PyObject* const* a, int device, LinearFp8Call& c, Matrix& x, Matri
   if (!matrix(a[0], device, x) || !matrix(a[1], device, xs) || !matrix(a[2], device, w) || !matrix(a[3], device, ws) || !matrix(a[4], device, out) ||
       !values8(x) || !values8(w) || !row_scales(xs, x) || !weight_scales(ws, w) || x.cols != w.cols || out.rows != x.rows)
     return false;
-  c.a = x.data; c.lda = x.ld; c.a_scales = xs.data; c.lda_s = xs.ld; c.w = w.data; c.ldw = w.ld; c.w_scales = (const float*)ws.data;
+  c.a = x.data; c.lda = x.ld; c.a_scales = xs.data; c.lda_s = xs.ld; c.w = w.data; c.ldw = w.ld; c.w_scales = ws.data;
   c.out = out.data; c.ldo = out.ld; c.m = (int)x.rows; c.n = (int)out.cols; c.k = (int)x.cols;
   return true;
 }
@@ -151,7 +145,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (out.type == at::kFloat) c.mode = add ? OUT_ADD : OUT_F32;
     else if (out.type == at::kBFloat16 && !add) c.mode = OUT_BF16;
     else return false;
-    c.status = (int*)status;
+    c.status = (void*)status;
     c.stream = (void*)stream;
     return launch(g_linear, c);
   });
@@ -178,7 +172,7 @@ PyObject* gated(PyObject*, PyObject* const* a, Py_ssize_t n) {
     c.gated = 1;
     c.act = (int)act;
     c.limit = (float)PyFloat_AS_DOUBLE(a[7]);
-    c.status = (int*)status;
+    c.status = (void*)status;
     c.stream = (void*)stream;
     return launch(g_linear, c);
   });

@@ -9,6 +9,7 @@
 #include <type_traits>
 
 #include "fp8.cuh"
+#include "fp8_calls.h"
 
 TLLM_DEFINE_LAST_ERROR
 
@@ -293,8 +294,8 @@ static int check_rows(const char* name, int rows, int width, const void* out, lo
 
 using namespace tllm;
 
-// Entry points take their arguments as one struct, which the caller packs in the order of the declaration.
-struct QuantizeCall { const void* x; long long ldx; void* out; long long ldo; void* scales; long long lds; int rows, width, dtype; void* stream; };
+// Entry points take their arguments as one struct; ..._layout() says how the interpreter packs it.
+extern "C" const char* tllm_quantize_fp8_layout() { return TLLM_QUANTIZE_FP8(TLLM_LETTER); }
 extern "C" int tllm_quantize_fp8(const QuantizeCall* c) {
   const auto [x, ldx, out, ldo, scales, lds, rows, width, dtype, stream] = *c;
   if (int e = check_rows("quantize_fp8", rows, width, out, ldo, lds)) return e;
@@ -320,7 +321,7 @@ extern "C" int tllm_quantize_fp8(const QuantizeCall* c) {
   return TLLM_OK;
 }
 
-struct RmsNormCall { const float *x, *w; void* out; long long ldo; void* scales; long long lds; const int* rows_idx; int rows, width; float eps; void* stream; };
+extern "C" const char* tllm_rms_norm_fp8_layout() { return TLLM_RMS_NORM_FP8(TLLM_LETTER); }
 extern "C" int tllm_rms_norm_fp8(const RmsNormCall* c) {
   const auto [x, w, out, ldo, scales, lds, rows_idx, rows, width, eps, stream] = *c;
   if (int e = check_rows("rms_norm_fp8", rows, width, out, ldo, lds)) return e;
@@ -337,11 +338,12 @@ extern "C" int tllm_rms_norm_fp8(const RmsNormCall* c) {
            : per == 4 ? rms_norm_rows_kernel<4, F> : warps <= NORM_WARPS ? rms_norm_rows_kernel<8, F> : rms_norm_wide_rows_kernel<F>;
   };
   auto kern = full ? pick(std::true_type()) : pick(std::false_type());
-  TLLM_LAUNCH("rms_norm_fp8", kern, rows, 32 * warps, 0, (cudaStream_t)stream, x, w, (uint8_t*)out, ldo, (uint8_t*)scales, lds, rows_idx, width, groups, eps, vec);
+  TLLM_LAUNCH("rms_norm_fp8", kern, rows, 32 * warps, 0, (cudaStream_t)stream, (const float*)x, (const float*)w, (uint8_t*)out, ldo, (uint8_t*)scales, lds,
+              (const int*)rows_idx, width, groups, eps, vec);
   return TLLM_OK;
 }
 
-struct QuantizeWeightCall { const void* w; long long ldw; void* out; long long ldo; float* scales; int rows, width, dtype; void* stream; };
+extern "C" const char* tllm_quantize_weight_fp8_layout() { return TLLM_QUANTIZE_WEIGHT_FP8(TLLM_LETTER); }
 extern "C" int tllm_quantize_weight_fp8(const QuantizeWeightCall* c) {
   const auto [w, ldw, out, ldo, scales, rows, width, dtype, stream] = *c;
   const int groups = (width + FP8_GROUP - 1) / FP8_GROUP;
@@ -353,8 +355,8 @@ extern "C" int tllm_quantize_weight_fp8(const QuantizeWeightCall* c) {
   cudaStream_t s = (cudaStream_t)stream;
   const dim3 grid(groups, row_blocks);
   if (dtype == TLLM_F32)
-    TLLM_LAUNCH("quantize_weight_fp8", quantize_weight_kernel<float>, grid, WEIGHT_THREADS, 0, s, (const float*)w, ldw, (uint8_t*)out, ldo, scales, rows, width, groups, vec);
+    TLLM_LAUNCH("quantize_weight_fp8", quantize_weight_kernel<float>, grid, WEIGHT_THREADS, 0, s, (const float*)w, ldw, (uint8_t*)out, ldo, (float*)scales, rows, width, groups, vec);
   else
-    TLLM_LAUNCH("quantize_weight_fp8", quantize_weight_kernel<__nv_bfloat16>, grid, WEIGHT_THREADS, 0, s, (const __nv_bfloat16*)w, ldw, (uint8_t*)out, ldo, scales, rows, width, groups, vec);
+    TLLM_LAUNCH("quantize_weight_fp8", quantize_weight_kernel<__nv_bfloat16>, grid, WEIGHT_THREADS, 0, s, (const __nv_bfloat16*)w, ldw, (uint8_t*)out, ldo, (float*)scales, rows, width, groups, vec);
   return TLLM_OK;
 }

@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "fp8.cuh"
+#include "fp8_calls.h"
 #include "tc_common.cuh"
 
 TLLM_DEFINE_LAST_ERROR
@@ -890,13 +891,11 @@ static int launch_few_rows(const Fp8Args& p, const void* a, long long lda, const
 
 using namespace tllm;
 
+extern "C" const char* tllm_linear_fp8_layout() { return TLLM_LINEAR_FP8(TLLM_LETTER); }
 // gated: `n` is the number of output columns, w has 256 * ceil(n / 128) rows; else w has n rows.
-struct LinearFp8Call {
-  const void* a; long long lda; const void* a_scales; long long lda_s; const void* w; long long ldw; const float* w_scales; void* out; long long ldo;
-  void* out_scales; long long ldo_s; int m, n, k, mode, gated, act; float limit; int* status; void* stream;
-};
 extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
-  const auto [a, lda, a_scales, lda_s, w, ldw, w_scales, out, ldo, out_scales, ldo_s, m, n, k, mode, gated, act, limit, status, stream] = *c;
+  const auto [a, lda, a_scales, lda_s, w, ldw, w_scales, out, ldo, out_scales, ldo_s, m, n, k, mode, gated, act, limit, status_word, stream] = *c;
+  int* status = (int*)status_word;
   TLLM_REQUIRE(m > 0 && n > 0 && k > 0, "linear_fp8: empty product");
   TLLM_REQUIRE((uintptr_t)a % 16 == 0 && (uintptr_t)w % 16 == 0 && lda % 16 == 0 && ldw % 16 == 0 && lda >= k && ldw >= k,
                "linear_fp8: rows of 8-bit values start on 16 bytes");
@@ -904,7 +903,7 @@ extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
   TLLM_REQUIRE(act >= 0 && act <= 3 && (act != ACT_CLAMPED || limit > 0.f), "linear_fp8: activation code %d, limit %g", act, (double)limit);
   Fp8Args p = {};
   p.a = (const uint8_t*)a; p.w = (const uint8_t*)w; p.lda = lda; p.ldw = ldw; p.k = k;
-  p.a_scales = (const uint8_t*)a_scales; p.w_scales = w_scales; p.out = out; p.out_scales = (uint8_t*)out_scales;
+  p.a_scales = (const uint8_t*)a_scales; p.w_scales = (const float*)w_scales; p.out = out; p.out_scales = (uint8_t*)out_scales;
   p.lda_s = lda_s; p.ldo = ldo; p.ldo_s = ldo_s;
   p.m = m; p.n = n; p.groups = (k + BK - 1) / BK;
   p.mode = mode; p.gate = make_gate(act, limit);

@@ -1530,13 +1530,10 @@ def weight_to_fp8(w: torch.Tensor):
     return out
 
 
-# The arguments of an entry point travel as one packed struct, in the order and with the types of its C declaration (P: pointer,
-# q: 64 bits, i: 32 bits, f: float): a call of a dozen ctypes objects takes longer than the small kernels.
-_FP8_ENTRIES = {name: (library, struct.Struct(layout)) for name, library, layout in (
-    ("tllm_quantize_fp8", "fp8_quantize", "PqPqPqiiiP"),
-    ("tllm_rms_norm_fp8", "fp8_quantize", "PPPqPqPiifP"),
-    ("tllm_quantize_weight_fp8", "fp8_quantize", "PqPqPiiiP"),
-    ("tllm_linear_fp8", "linear_fp8", "PqPqPqPPqPqiiiiiifPP"))}
+# The arguments of an entry point travel as one packed struct, as its library says (csrc/fp8_calls.h): a call of a dozen ctypes objects
+# takes longer than the small kernels.
+_FP8_ENTRIES = {"tllm_quantize_fp8": "fp8_quantize", "tllm_rms_norm_fp8": "fp8_quantize", "tllm_quantize_weight_fp8": "fp8_quantize",
+                "tllm_linear_fp8": "linear_fp8"}
 _fp8_loaded = {}
 
 # The same calls without the interpreter (csrc/fp8_calls.cpp), for a call whose arguments are all ordinary: None until the first
@@ -1554,7 +1551,7 @@ def _fp8_load_native() -> None:
         print(f"[tiny_llm_b200] 8-bit calls go through the interpreter: {e}", file=sys.stderr, flush=True)
         _fp8_native = False
         return
-    module.bind(*(ctypes.cast(getattr(build.load_library(library), name), ctypes.c_void_p).value for name, (library, _) in _FP8_ENTRIES.items()))
+    module.bind(*(ctypes.cast(getattr(build.load_library(library), name), ctypes.c_void_p).value for name, library in _FP8_ENTRIES.items()))
     _fp8_native = module
 
 
@@ -1563,9 +1560,10 @@ def _fp8_call(name: str, *args) -> None:
         _fp8_load_native()
     got = _fp8_loaded.get(name)
     if got is None:
-        library, layout = _FP8_ENTRIES[name]
-        lib = build.load_library(library)
-        got = _fp8_loaded[name] = (lib, getattr(lib, name), layout.pack)
+        lib = build.load_library(_FP8_ENTRIES[name])
+        layout = getattr(lib, name + "_layout")
+        layout.restype = ctypes.c_char_p
+        got = _fp8_loaded[name] = (lib, getattr(lib, name), struct.Struct(layout().decode()).pack)
     _call(got[0], got[1], got[2](*args))
 
 

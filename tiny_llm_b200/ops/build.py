@@ -25,7 +25,7 @@ HEADERS = ["common.cuh", "per_device.h"]
 EXTRA_HEADERS = {"sampling": ["sampling_noalloc.h"], "attention_mma": ["attention_tiles.cuh"],
                  "attention_maps_mma": ["attention_tiles.cuh"], "attention_talk_mma": ["attention_tiles.cuh"],
                  "linear_tc": ["tc_common.cuh"], "linear_generic": ["tc_common.cuh"], "linear_f32_tc": ["tc_common.cuh"], "delta_rule": ["tc_common.cuh"],
-                 "linear_fp8": ["tc_common.cuh", "fp8.cuh"], "fp8_quantize": ["fp8.cuh"],
+                 "linear_fp8": ["tc_common.cuh", "fp8.cuh", "fp8_calls.h"], "fp8_quantize": ["fp8.cuh", "fp8_calls.h"], "fp8_calls": ["fp8_calls.h"],
                  "attention_tc": ["tc_common.cuh"], "attention_decode": ["tc_common.cuh"], "attention_generic": ["attention_route.h"],
                  "window_attention": ["window_attention.cuh"], "window_attention_mma": ["window_attention.cuh"]}   # per-source headers that enter the hash
 
@@ -146,8 +146,9 @@ def compile_extension(name: str, verbose: bool = True) -> str:
     flags = ["-O2", "-std=c++17", "-shared", "-fPIC", "-I", os.path.join(root, "include"), "-I", include]
     source = os.path.join(CSRC, name + ".cpp")
     h = hashlib.sha256()
-    with open(source, "rb") as fh:
-        h.update(fh.read())
+    for path in [source] + [os.path.join(CSRC, f) for f in EXTRA_HEADERS.get(name, [])]:
+        with open(path, "rb") as fh:
+            h.update(fh.read())
     h.update(" ".join(flags + [torch.__version__, sys.version]).encode())
     out = os.path.join(build_dir(), f"{name}-{h.hexdigest()[:16]}.so")
     if os.path.isfile(out):
@@ -159,7 +160,7 @@ def compile_extension(name: str, verbose: bool = True) -> str:
     if verbose:
         print(f"[tiny_llm_b200] compiling {name}.cpp ...", file=sys.stderr, flush=True)
     lib = os.path.join(root, "lib")
-    proc = subprocess.run([compiler] + flags + ["-o", tmp, source, "-L", lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", f"-Wl,-rpath,{lib}"],
+    proc = subprocess.run([compiler] + flags + ["-I", CSRC, "-o", tmp, source, "-L", lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", f"-Wl,-rpath,{lib}"],
                           stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if proc.returncode != 0:
         raise BuildError(f"the host compiler failed on {name}.cpp:\n{proc.stdout}")
