@@ -159,6 +159,25 @@ def test_arguments_have_one_layout():
         assert len(letters()) == fields and struct.calcsize(letters().decode()) == size
 
 
+def test_sizes_next_to_32_bits_are_refused():
+    """Tiles, runs and groups are rounded up in 32 bits: the entry points refuse what that would carry over, before they look at a device."""
+    most = 2 ** 31 - 4096
+    at = 1 << 20
+    entries = {
+        "tllm_quantize_fp8": lambda m, k: (at, k, at, 16 * (k // 16 + 1), at, k // 128 + 1, m, k, 0, 0),
+        "tllm_rms_norm_fp8": lambda m, k: (at, at, at, 16 * (k // 16 + 1), at, k // 128 + 1, 0, m, k, 1e-5, 0),
+        "tllm_quantize_weight_fp8": lambda m, k: (at, k, at, 16 * (k // 16 + 1), at, m, k, 0, 0)}
+    for name, args in entries.items():
+        for m, k in ((1, most + 1), (1, 2 ** 31 - 1), (most + 1, 16), (2 ** 31 - 1, 128)):
+            with pytest.raises(KernelError, match=f"at most {most} rows"):
+                ops._fp8_call(name, *args(m, k))
+        with pytest.raises(KernelError, match="32 bits"):
+            ops._fp8_call(name, *args(2 ** 31, 128))
+    for m, n, k, gated in ((most + 1, 8, 8, 0), (8, most + 1, 8, 0), (8, 8, 2 ** 31 - 1, 0), (8, 2 ** 30 + 1, 8, 1), (8, 2 ** 31 - 1, 8, 1)):
+        with pytest.raises(KernelError, match=f"at most {most} rows"):
+            ops._fp8_call("tllm_linear_fp8", at, 16 * (k // 16 + 1), at, k // 128 + 1, at, 16 * (k // 16 + 1), at, at, n, 0, 0, m, n, k, 0, gated, 0, 0.0, at, 0)
+
+
 def test_threads_that_load_the_extension_at_once_get_one_module(monkeypatch, tmp_path):
     """In a fresh build folder, with a compiler that takes its time, so that they do meet."""
     import shutil

@@ -13,6 +13,7 @@
 namespace tllm {
 
 constexpr int FP8_GROUP = 128;
+constexpr int FP8_MOST = 0x7FFFFFFF - 4095;    // rows or values of a row: the kernels round them up to whole tiles, runs and groups in 32 bits
 
 // The scale's biased exponent (what e8m0 holds; 255 is NaN) from the bits of the largest magnitude (maximum as integers, which
 // puts NaN above infinity above the finite values).

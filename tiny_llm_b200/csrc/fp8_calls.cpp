@@ -22,7 +22,7 @@ int (*g_linear)(const LinearFp8Call*) = nullptr;
 
 constexpr int F32 = 0, BF16 = 1;
 constexpr int OUT_BF16 = 0, OUT_F32 = 1, OUT_ADD = 2, OUT_FP8 = 3;
-constexpr int64_t MOST = INT32_MAX - 256;
+constexpr int64_t MOST = INT32_MAX - 4095;
 
 // A matrix of rows on the wanted device; false: not an ordinary one.
 struct Matrix { void* data; int64_t rows, cols, ld; c10::ScalarType type; };

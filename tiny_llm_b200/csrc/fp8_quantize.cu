@@ -285,8 +285,9 @@ quantize_weight_kernel(const T* __restrict__ w, long long ldw, uint8_t* __restri
 
 static int check_rows(const char* name, int rows, int width, const void* out, long long ldo, long long lds) {
   TLLM_REQUIRE(rows > 0 && width > 0, "%s: empty input", name);
+  TLLM_REQUIRE(rows <= FP8_MOST && width <= FP8_MOST, "%s: at most %d rows and values per row", name, FP8_MOST);
   TLLM_REQUIRE((uintptr_t)out % 16 == 0 && ldo % 16 == 0 && ldo >= width, "%s: rows of 8-bit values start on 16 bytes", name);
-  TLLM_REQUIRE(lds >= (width + FP8_GROUP - 1) / FP8_GROUP, "%s: a row of scales holds one per group of 128", name);
+  TLLM_REQUIRE(lds >= (width + 127ll) / 128, "%s: a row of scales holds one per group of 128", name);
   return TLLM_OK;
 }
 
@@ -346,8 +347,8 @@ extern "C" int tllm_rms_norm_fp8(const RmsNormCall* c) {
 extern "C" const char* tllm_quantize_weight_fp8_layout() { return TLLM_QUANTIZE_WEIGHT_FP8(TLLM_LETTER); }
 extern "C" int tllm_quantize_weight_fp8(const QuantizeWeightCall* c) {
   const auto [w, ldw, out, ldo, scales, rows, width, dtype, stream] = *c;
+  if (int e = check_rows("quantize_weight_fp8", rows, width, out, ldo, (width + 127ll) / 128)) return e;
   const int groups = (width + FP8_GROUP - 1) / FP8_GROUP;
-  if (int e = check_rows("quantize_weight_fp8", rows, width, out, ldo, groups)) return e;
   const int row_blocks = (rows + FP8_GROUP - 1) / FP8_GROUP;
   TLLM_REQUIRE(row_blocks <= 65535, "quantize_weight_fp8: %d rows are too many for one launch", rows);
   const int bytes = dtype == TLLM_F32 ? 16 : 8;

@@ -897,6 +897,7 @@ extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
   const auto [a, lda, a_scales, lda_s, w, ldw, w_scales, out, ldo, out_scales, ldo_s, m, n, k, mode, gated, act, limit, status_word, stream] = *c;
   int* status = (int*)status_word;
   TLLM_REQUIRE(m > 0 && n > 0 && k > 0, "linear_fp8: empty product");
+  TLLM_REQUIRE(m <= FP8_MOST && n <= (gated ? FP8_MOST / 2 : FP8_MOST) && k <= FP8_MOST, "linear_fp8: at most %d rows of either operand and values per row", FP8_MOST);
   TLLM_REQUIRE((uintptr_t)a % 16 == 0 && (uintptr_t)w % 16 == 0 && lda % 16 == 0 && ldw % 16 == 0 && lda >= k && ldw >= k,
                "linear_fp8: rows of 8-bit values start on 16 bytes");
   TLLM_REQUIRE(gated ? (mode == OUT_BF16 || mode == OUT_FP8) : (mode >= OUT_BF16 && mode <= OUT_ADD), "linear_fp8: output code %d", mode);

@@ -1564,7 +1564,11 @@ def _fp8_call(name: str, *args) -> None:
         layout = getattr(lib, name + "_layout")
         layout.restype = ctypes.c_char_p
         got = _fp8_loaded[name] = (lib, getattr(lib, name), struct.Struct(layout().decode()).pack)
-    _call(got[0], got[1], got[2](*args))
+    try:
+        packed = got[2](*args)
+    except struct.error as e:
+        raise KernelError(f"{name[5:]}: sizes that 32 bits do not hold") from e
+    _call(got[0], got[1], packed)
 
 
 def _fp8_here(name: str, *tensors) -> int:
