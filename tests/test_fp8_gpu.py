@@ -543,3 +543,28 @@ def test_gated_scales_whose_product_is_no_normal_float(ops, m, i):
     assert not bool(torch.isnan(out).any())
     assert bool(((out.double() - want).abs() <= off + 2.0 ** -8 * (want.abs() + off) + 4 * 2.0 ** -149 * (up.abs() + 1) + 2.0 ** -133)[~beyond].all())
     ops.check_status()
+
+
+@pytest.mark.parametrize("m", [1, 20, 40])
+def test_more_than_65535_blocks_of_columns(ops, m):
+    g = rng(m)
+    n, k = 65536 * 128 + 5, 16
+    a, w = rows8(ops, randn(g, m, k)), weight8(ops, randn(g, n, k))
+    last = slice(65534 * 128, n)
+    out = torch.empty(m, n, dtype=torch.bfloat16, device=DEV)
+    ops.linear_fp8(*a, *w, out)
+    for part in (slice(0, 300), last):
+        scales = w[1][part.start // 128: -(-part.stop // 128)]
+        want, off = fu.product(*a, w[0][part], scales)
+        assert bool(((out[:, part].double() - want).abs() <= off + 2.0 ** -8 * (want.abs() + off)).all())
+    ops.check_status()
+
+
+def test_weights_of_more_than_65535_blocks_of_rows(ops):
+    g = rng(1)
+    n, k = 65536 * 128 + 5, 16
+    x = randn(g, n, k)
+    data, scales = weight8(ops, x)
+    for part in (slice(0, 300 * 128), slice(65530 * 128, n)):
+        want, ws = fu.quantize_weight(x[part])
+        assert same(data[part], want) and same(scales[part.start // 128: -(-part.stop // 128)], ws)

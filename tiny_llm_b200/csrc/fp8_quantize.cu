@@ -251,7 +251,9 @@ quantize_weight_kernel(const T* __restrict__ w, long long ldw, uint8_t* __restri
   __shared__ uint32_t most[WARPS];
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int k = blockIdx.x * FP8_GROUP + 4 * lane, n0 = blockIdx.y * FP8_GROUP + warp;
+  const int row_block = blockIdx.z * gridDim.y + blockIdx.y;
+  if (row_block > (rows - 1) / FP8_GROUP) return;
+  const int k = blockIdx.x * FP8_GROUP + 4 * lane, n0 = row_block * FP8_GROUP + warp;
   Held<T> held[PER];
   const T* src = w + (long long)n0 * ldw;
 #pragma unroll
@@ -278,7 +280,7 @@ quantize_weight_kernel(const T* __restrict__ w, long long ldw, uint8_t* __restri
     give(held[i], v);
     if (n0 + i * WARPS < rows) store4(dst + (long long)i * WARPS * ldo, k, width, fp8_pack4(v[0], v[1], v[2], v[3], inverse, byte));
   }
-  if (threadIdx.x == 0) scales[(size_t)blockIdx.y * groups + blockIdx.x] = fp8_scale(byte);
+  if (threadIdx.x == 0) scales[(size_t)row_block * groups + blockIdx.x] = fp8_scale(byte);
   __syncthreads();
   if (threadIdx.x == 0) __threadfence();
 }
@@ -350,11 +352,11 @@ extern "C" int tllm_quantize_weight_fp8(const QuantizeWeightCall* c) {
   if (int e = check_rows("quantize_weight_fp8", rows, width, out, ldo, (width + 127ll) / 128)) return e;
   const int groups = (width + FP8_GROUP - 1) / FP8_GROUP;
   const int row_blocks = (rows + FP8_GROUP - 1) / FP8_GROUP;
-  TLLM_REQUIRE(row_blocks <= 65535, "quantize_weight_fp8: %d rows are too many for one launch", rows);
   const int bytes = dtype == TLLM_F32 ? 16 : 8;
   const int vec = (uintptr_t)w % bytes == 0 && ldw % 4 == 0;
   cudaStream_t s = (cudaStream_t)stream;
-  const dim3 grid(groups, row_blocks);
+  const int most = 65535, grid_z = (row_blocks + most - 1) / most;      // (what a grid's second side holds)
+  const dim3 grid(groups, (row_blocks + grid_z - 1) / grid_z, grid_z);
   if (dtype == TLLM_F32)
     TLLM_LAUNCH("quantize_weight_fp8", quantize_weight_kernel<float>, grid, WEIGHT_THREADS, 0, s, (const float*)w, ldw, (uint8_t*)out, ldo, (float*)scales, rows, width, groups, vec);
   else

@@ -929,22 +929,23 @@ extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
   //   4,096 x 4,096 of 256 13.4 / 14.7 / 20, 512 20 / 14.8 / 20, 1,024 40 / 27 / 21
   //   4,096 x 14,336 of 128 18.7 / 40 / 53, 256 32 / 40 / 53, 512 58 / 40 / 53, 1,024 116 / 78 / 59
   // gated, few / 128 x 256: 5,632 x 2,048 of 64 rows 10.7 / 14.9, 128 14.2 / 15.4, 256 29 / 16; 14,336 x 4,096 of 64 23.7 / 26.4, 128 45 / 28
+  // (The columns' blocks are the second side of few's grid, which holds 65,535.)
   const long long w_values = (long long)w_rows * k;
   auto fits = [&p, w_tiles, w_values](int rows, int resident) {
     const long long parts = (p.m + rows - 1) / rows;
-    return p.m <= rows || (parts * w_values <= 36000000 && parts * w_tiles <= 148 * resident);
+    return w_tiles <= 65535 && (p.m <= rows || (parts * w_values <= 36000000 && parts * w_tiles <= 148 * resident));
   };
 #define TLLM_FEW(BN, STAGES, WHOLE, GATED, HALVES) return launch_few_rows<BN, STAGES, WHOLE, GATED, HALVES>(p, a, lda, w, ldw, w_rows, k, status, s)
 #define TLLM_TILES(BN, STAGES, GATED) return launch_tiles<BN, STAGES, GATED>(p, a, lda, w, ldw, w_rows, k, status, s)
   if (gated) {
     if (fits(16, 1)) TLLM_FEW(16, 2, 3, true, 1);
     if (fits(32, 1)) TLLM_FEW(32, 4, 5, true, 1);
-    if (m <= 64 || ((m + 63) / 64) * w_tiles <= 148) TLLM_FEW(64, 3, 5, true, 2);
+    if ((m <= 64 && w_tiles <= 65535) || ((m + 63) / 64) * w_tiles <= 148) TLLM_FEW(64, 3, 5, true, 2);
     TLLM_TILES(256, 4, true);
   }
   if (fits(16, 1)) TLLM_FEW(16, 5, 6, false, 1);
   if (fits(32, 2)) TLLM_FEW(32, 4, 5, false, 1);
-  if (m <= 64) TLLM_FEW(64, 3, 4, false, 2);
+  if (m <= 64 && w_tiles <= 65535) TLLM_FEW(64, 3, 4, false, 2);
   if (((m + 127) / 128) * w_tiles <= 74) TLLM_FEW(128, 4, 6, false, 4);
   if (((m + 127) / 128) * (long long)((n + 255) / 256) >= 74) TLLM_TILES(256, 4, false);
   TLLM_TILES(128, 6, false);
