@@ -241,8 +241,8 @@ __device__ __forceinline__ void take(Held<__nv_bfloat16>& h, const __nv_bfloat16
 }
 
 // A CTA per block of 128 x 128, which stays in registers (bfloat16 as it came) between the search for its largest magnitude and the
-// rounding.  The products may begin to read a weight while earlier launches still run, so this kernel never lets the next one start
-// early, and its values are in memory before it ends.
+// rounding.  The products may begin to read a weight, through the copy unit, before their wait for earlier launches: this kernel never lets
+// the next one start early, and its values are in memory, for the copy unit too, before it ends.
 template <typename T>
 __global__ void __launch_bounds__(WEIGHT_THREADS, 3)
 quantize_weight_kernel(const T* __restrict__ w, long long ldw, uint8_t* __restrict__ out, long long ldo, float* __restrict__ scales,
@@ -251,9 +251,7 @@ quantize_weight_kernel(const T* __restrict__ w, long long ldw, uint8_t* __restri
   __shared__ uint32_t most[WARPS];
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row_block = blockIdx.z * gridDim.y + blockIdx.y;
-  if (row_block > (rows - 1) / FP8_GROUP) return;
-  const int k = blockIdx.x * FP8_GROUP + 4 * lane, n0 = row_block * FP8_GROUP + warp;
+  const int k = blockIdx.x * FP8_GROUP + 4 * lane, n0 = blockIdx.y * FP8_GROUP + warp;
   Held<T> held[PER];
   const T* src = w + (long long)n0 * ldw;
 #pragma unroll
@@ -280,7 +278,7 @@ quantize_weight_kernel(const T* __restrict__ w, long long ldw, uint8_t* __restri
     give(held[i], v);
     if (n0 + i * WARPS < rows) store4(dst + (long long)i * WARPS * ldo, k, width, fp8_pack4(v[0], v[1], v[2], v[3], inverse, byte));
   }
-  if (threadIdx.x == 0) scales[(size_t)row_block * groups + blockIdx.x] = fp8_scale(byte);
+  if (threadIdx.x == 0) scales[(size_t)blockIdx.y * groups + blockIdx.x] = fp8_scale(byte);
   __syncthreads();
   if (threadIdx.x == 0) __threadfence();
 }
@@ -351,15 +349,20 @@ extern "C" int tllm_quantize_weight_fp8(const QuantizeWeightCall* c) {
   const auto [w, ldw, out, ldo, scales, rows, width, dtype, stream] = *c;
   if (int e = check_rows("quantize_weight_fp8", rows, width, out, ldo, (width + 127ll) / 128)) return e;
   const int groups = (width + FP8_GROUP - 1) / FP8_GROUP;
-  const int row_blocks = (rows + FP8_GROUP - 1) / FP8_GROUP;
-  const int bytes = dtype == TLLM_F32 ? 16 : 8;
-  const int vec = (uintptr_t)w % bytes == 0 && ldw % 4 == 0;
+  const int bytes = dtype == TLLM_F32 ? 4 : 2;
+  const int vec = (uintptr_t)w % (4 * bytes) == 0 && ldw % 4 == 0;
   cudaStream_t s = (cudaStream_t)stream;
-  const int most = 65535, grid_z = (row_blocks + most - 1) / most;      // (what a grid's second side holds)
-  const dim3 grid(groups, (row_blocks + grid_z - 1) / grid_z, grid_z);
-  if (dtype == TLLM_F32)
-    TLLM_LAUNCH("quantize_weight_fp8", quantize_weight_kernel<float>, grid, WEIGHT_THREADS, 0, s, (const float*)w, ldw, (uint8_t*)out, ldo, (float*)scales, rows, width, groups, vec);
-  else
-    TLLM_LAUNCH("quantize_weight_fp8", quantize_weight_kernel<__nv_bfloat16>, grid, WEIGHT_THREADS, 0, s, (const __nv_bfloat16*)w, ldw, (uint8_t*)out, ldo, (float*)scales, rows, width, groups, vec);
+  constexpr int MOST_ROWS = 65535 * FP8_GROUP;      // of a launch: the second side of its grid (working the third one in cost every launch 5 to 10 %)
+  for (long long r = 0; r < rows; r += MOST_ROWS) {
+    const int some = rows - r < MOST_ROWS ? (int)(rows - r) : MOST_ROWS;
+    const dim3 grid(groups, (some + FP8_GROUP - 1) / FP8_GROUP);
+    const uint8_t* from = (const uint8_t*)w + r * ldw * bytes;
+    uint8_t* to = (uint8_t*)out + r * ldo;
+    float* to_scales = (float*)scales + r / FP8_GROUP * groups;
+    if (dtype == TLLM_F32)
+      TLLM_LAUNCH("quantize_weight_fp8", quantize_weight_kernel<float>, grid, WEIGHT_THREADS, 0, s, (const float*)from, ldw, to, ldo, to_scales, some, width, groups, vec);
+    else
+      TLLM_LAUNCH("quantize_weight_fp8", quantize_weight_kernel<__nv_bfloat16>, grid, WEIGHT_THREADS, 0, s, (const __nv_bfloat16*)from, ldw, to, ldo, to_scales, some, width, groups, vec);
+  }
   return TLLM_OK;
 }
