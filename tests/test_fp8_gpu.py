@@ -568,3 +568,19 @@ def test_weights_of_more_than_65535_blocks_of_rows(ops):
     for part in (slice(0, 300 * 128), slice(65530 * 128, n)):
         want, ws = fu.quantize_weight(x[part])
         assert same(data[part], want) and same(scales[part.start // 128: -(-part.stop // 128)], ws)
+
+
+@pytest.mark.parametrize("m", [3, 40, 64, 100, 700])
+def test_gated_weights_may_be_made_right_before_they_are_read(ops, m):
+    g = rng(m)
+    i, k = 2500, 1024
+    x = [randn(g, 256 * fu.groups(i), k) / math.sqrt(k) for _ in range(4)]
+    a, room = rows8(ops, randn(g, m, k)), ops.fp8_weight(256 * fu.groups(i), k, DEV)
+    out = [torch.empty(m, i, dtype=torch.bfloat16, device=DEV) for _ in x]
+    for w, o in zip(x, out):
+        ops.quantize_weight_fp8(w, *room)
+        ops.linear_swiglu_fp8(*a, *room, o)
+    for w, o in zip(x, out):
+        want, off = fu.gated(*a, *weight8(ops, w), i, "silu")
+        assert bool(((o.double() - want).abs() <= off + 2.0 ** -8 * (want.abs() + off)).all())
+    ops.check_status()

@@ -280,7 +280,10 @@ quantize_weight_kernel(const T* __restrict__ w, long long ldw, uint8_t* __restri
   }
   if (threadIdx.x == 0) scales[(size_t)blockIdx.y * groups + blockIdx.x] = fp8_scale(byte);
   __syncthreads();
-  if (threadIdx.x == 0) __threadfence();
+  if (threadIdx.x == 0) {      // (behind the barrier, so for all threads' values)
+    __threadfence();
+    asm volatile("fence.proxy.async.global;" ::: "memory");
+  }
 }
 
 static int check_rows(const char* name, int rows, int width, const void* out, long long ldo, long long lds) {
