@@ -584,3 +584,46 @@ def test_gated_weights_may_be_made_right_before_they_are_read(ops, m):
         want, off = fu.gated(*a, *weight8(ops, w), i, "silu")
         assert bool(((o.double() - want).abs() <= off + 2.0 ** -8 * (want.abs() + off)).all())
     ops.check_status()
+
+
+# ---------------------------------------------------------------------------------------------- which kernel
+
+
+def kernel_of(m, n, k, gated=False):
+    """(which kernel, whether K is cut) of a product of these sizes: 16 to 128 are the rows of A beside a block of columns, 1,128 and 1,256 the
+    kernels of large tiles."""
+    import ctypes
+    from tiny_llm_b200.ops import build
+    slices = ctypes.c_int(0)
+    kernel = build.load_library("linear_fp8").tllm_linear_fp8_kernel(m, n, k, int(gated), ctypes.byref(slices))
+    return kernel, slices.value > 1
+
+
+@pytest.mark.parametrize("kernel,cut,m,n,k", [
+    (16, False, 9, 300, 500), (16, True, 13, 1000, 2100), (16, True, 100, 500, 1100), (32, False, 60, 9000, 400), (32, True, 50, 4100, 4001),
+    (64, False, 40, 19000, 129), (64, False, 64, 19001, 1000), (64, True, 50, 2050, 9000), (64, True, 64, 4096, 14336), (128, True, 100, 1300, 7000),
+    (128, True, 128, 4100, 2305), (128, True, 200, 2000, 4001), (128, True, 300, 1001, 4000), (1128, False, 300, 4100, 520), (1128, False, 513, 2200, 1001),
+    (1128, False, 257, 4300, 129), (1256, False, 1030, 4001, 1000), (1256, False, 2100, 1290, 2000)])
+def test_products_of_each_kernel(ops, kernel, cut, m, n, k):
+    """What test_products_are_near_64_bits looks at, with the tails of K and of the columns, rows that do not start on 16 bytes and every kind of
+    output, on the kernel that is named."""
+    assert kernel_of(m, n, k) == (kernel, cut)
+    test_products_are_near_64_bits(ops, m, n, k)
+
+
+@pytest.mark.parametrize("act,limit", [("silu", 0.0), ("clamped", 1.5)])
+@pytest.mark.parametrize("kernel,cut,m,i,k", [
+    (16, False, 12, 300, 500), (16, True, 8, 1000, 2048), (16, True, 16, 1000, 2100), (16, True, 3, 5632, 2048), (32, False, 40, 6400, 300), (32, True, 64, 2000, 3001),
+    (64, False, 64, 10001, 300), (64, True, 64, 1500, 7000), (64, False, 200, 4000, 700), (64, True, 100, 1000, 9001),
+    (1256, False, 700, 2501, 650), (1256, False, 1300, 1290, 1111), (1256, False, 513, 5632, 2048)])
+def test_gated_products_of_each_kernel(ops, kernel, cut, m, i, k, act, limit):
+    assert kernel_of(m, i, k, gated=True) == (kernel, cut)
+    test_gated_products(ops, m, i, k, act, limit)
+
+
+def test_the_kernels_of_the_other_tests(ops):
+    """The sizes by which the tests above mean a kernel."""
+    assert [kernel_of(m, n, k)[0] for m, n, k in [(4, 130, 300), (5, 700, 1100), (40, 14336, 300), (64, 40000, 300), (128, 4096, 2304), (600, 3000, 300), (700, 8192, 400)]] == \
+        [16, 16, 32, 64, 128, 1128, 1256]
+    assert [kernel_of(m, i, 300, gated=True)[0] for m, i in [(4, 130), (40, 6400), (64, 14336), (700, 2500)]] == [16, 32, 64, 1256]
+    assert [kernel_of(m, 1792, 128, gated=True)[0] for m in (3, 100, 2400)] == [16, 16, 1256]

@@ -887,6 +887,37 @@ static int launch_few_rows(const Fp8Args& p, const void* a, long long lda, const
   return launch_few<BN, STAGES, GATED, HALVES, true, BN + 8>(p, f, a, lda, w, ldw, w_rows, k, status, s);
 }
 
+// Few rows of A, or so few tiles that K has to be cut to fill the SMs: the weight's 128 rows as the large side (few), with as many rows
+// of A beside them as keep what the CTAs fetch of the weight within 36 MB and them at once on the SMs (16 rows: one per SM): small tiles have the shorter
+// way from the first product to the last store.  Otherwise tiles of 128 x 256 when they fill half the SMs, else of 128 x 128.
+// us, few with 16 / 32 / 64 / 128 rows (columns x values of K):
+//   2,560 x 2,048 of 32 rows 3.8 / 4.7 / 5.6 / 5.8, 64 4.8 / 5.0 / 6.2 / 5.8, 128 6.5 / 6.0 / 6.8 / 6.7, 256 12.2 / 8.6 / 8.6 / 8.4
+//   4,096 x 4,096 of 64 7.8 / 7.1 / 8.3 / 8.2; 4,096 x 14,336 of 64 18.8 / 15.3 / 13.8 / 16.6
+//   300 x 300 of 300 3.0 / 3.7 / 4.3 / 6.1; 1,000 x 1,520 of 333 6.3 / 5.8 / 7.1 / 6.7; 1,000 x 1,000 of 1,000 12.1 / 6.8 / 8.0 / 7.8
+//   gated 5,632 x 2,048 of 32 8.4 / 8.1 / 9.1, 64 11.2 / 10.6 / 10.2; 300 x 300 of 300 4.5 / 5.4 / 6.8
+// few / 128 x 128 / 128 x 256:
+//   2,560 x 2,048 of 128 rows 7.1 / 9.6 / 13.4, 256 8.9 / 9.4 / 13.4, 512 11.2 / 9.8 / 13.7, 1,024 25 / 17.4 / 14.3
+//   4,096 x 4,096 of 256 13.4 / 14.7 / 20, 512 20 / 14.8 / 20, 1,024 40 / 27 / 21
+//   4,096 x 14,336 of 128 18.7 / 40 / 53, 256 32 / 40 / 53, 512 58 / 40 / 53, 1,024 116 / 78 / 59
+// gated, few / 128 x 256: 5,632 x 2,048 of 64 rows 10.7 / 14.9, 128 14.2 / 15.4, 256 29 / 16; 14,336 x 4,096 of 64 23.7 / 26.4, 128 45 / 28
+// (The columns' blocks are the second side of few's grid, which holds 65,535.)
+// (Few: the rows of A per tile; tiles: 1,000 and their columns.)
+enum Kernel { FEW_16 = 16, FEW_32 = 32, FEW_64 = 64, FEW_128 = 128, TILES_128 = 1128, TILES_256 = 1256 };
+static Kernel pick_kernel(const Fp8Args& p, bool gated) {
+  const long long m = p.m, w_tiles = (p.n + 127) / 128, w_values = (long long)p.w_rows * p.k;
+  auto fits = [m, w_tiles, w_values](int rows, int resident) {
+    const long long parts = (m + rows - 1) / rows;
+    return w_tiles <= 65535 && (m <= rows || (parts * w_values <= 36000000 && parts * w_tiles <= 148 * resident));
+  };
+  const bool some = m <= 64 && w_tiles <= 65535;
+  if (fits(16, 1)) return FEW_16;
+  if (fits(32, gated ? 1 : 2)) return FEW_32;
+  if (gated) return some || (m + 63) / 64 * w_tiles <= 148 ? FEW_64 : TILES_256;
+  if (some) return FEW_64;
+  if ((m + 127) / 128 * w_tiles <= 74) return FEW_128;
+  return (m + 127) / 128 * ((p.n + 255) / 256) >= 74 ? TILES_256 : TILES_128;
+}
+
 }  // namespace tllm
 
 using namespace tllm;
@@ -915,40 +946,29 @@ extern "C" int tllm_linear_fp8(const LinearFp8Call* c) {
   cudaStream_t s = (cudaStream_t)stream;
   const int w_rows = gated ? 256 * ((n + 127) / 128) : n;
   p.w_rows = w_rows;
-  const long long w_tiles = (n + 127) / 128;
-  // Few rows of A, or so few tiles that K has to be cut to fill the SMs: the weight's 128 rows as the large side (few), with as many rows
-  // of A beside them as keep what the CTAs fetch of the weight within 36 MB and them at once on the SMs (16 rows: one per SM): small tiles have the shorter
-  // way from the first product to the last store.  Otherwise tiles of 128 x 256 when they fill half the SMs, else of 128 x 128.
-  // us, few with 16 / 32 / 64 / 128 rows (columns x values of K):
-  //   2,560 x 2,048 of 32 rows 3.8 / 4.7 / 5.6 / 5.8, 64 4.8 / 5.0 / 6.2 / 5.8, 128 6.5 / 6.0 / 6.8 / 6.7, 256 12.2 / 8.6 / 8.6 / 8.4
-  //   4,096 x 4,096 of 64 7.8 / 7.1 / 8.3 / 8.2; 4,096 x 14,336 of 64 18.8 / 15.3 / 13.8 / 16.6
-  //   300 x 300 of 300 3.0 / 3.7 / 4.3 / 6.1; 1,000 x 1,520 of 333 6.3 / 5.8 / 7.1 / 6.7; 1,000 x 1,000 of 1,000 12.1 / 6.8 / 8.0 / 7.8
-  //   gated 5,632 x 2,048 of 32 8.4 / 8.1 / 9.1, 64 11.2 / 10.6 / 10.2; 300 x 300 of 300 4.5 / 5.4 / 6.8
-  // few / 128 x 128 / 128 x 256:
-  //   2,560 x 2,048 of 128 rows 7.1 / 9.6 / 13.4, 256 8.9 / 9.4 / 13.4, 512 11.2 / 9.8 / 13.7, 1,024 25 / 17.4 / 14.3
-  //   4,096 x 4,096 of 256 13.4 / 14.7 / 20, 512 20 / 14.8 / 20, 1,024 40 / 27 / 21
-  //   4,096 x 14,336 of 128 18.7 / 40 / 53, 256 32 / 40 / 53, 512 58 / 40 / 53, 1,024 116 / 78 / 59
-  // gated, few / 128 x 256: 5,632 x 2,048 of 64 rows 10.7 / 14.9, 128 14.2 / 15.4, 256 29 / 16; 14,336 x 4,096 of 64 23.7 / 26.4, 128 45 / 28
-  // (The columns' blocks are the second side of few's grid, which holds 65,535.)
-  const long long w_values = (long long)w_rows * k;
-  auto fits = [&p, w_tiles, w_values](int rows, int resident) {
-    const long long parts = (p.m + rows - 1) / rows;
-    return w_tiles <= 65535 && (p.m <= rows || (parts * w_values <= 36000000 && parts * w_tiles <= 148 * resident));
-  };
 #define TLLM_FEW(BN, STAGES, WHOLE, GATED, HALVES) return launch_few_rows<BN, STAGES, WHOLE, GATED, HALVES>(p, a, lda, w, ldw, w_rows, k, status, s)
 #define TLLM_TILES(BN, STAGES, GATED) return launch_tiles<BN, STAGES, GATED>(p, a, lda, w, ldw, w_rows, k, status, s)
-  if (gated) {
-    if (fits(16, 1)) TLLM_FEW(16, 2, 3, true, 1);
-    if (fits(32, 1)) TLLM_FEW(32, 4, 5, true, 1);
-    if ((m <= 64 && w_tiles <= 65535) || ((m + 63) / 64) * w_tiles <= 148) TLLM_FEW(64, 3, 5, true, 2);
-    TLLM_TILES(256, 4, true);
+  switch (pick_kernel(p, gated)) {
+    case FEW_16: if (gated) TLLM_FEW(16, 2, 3, true, 1); else TLLM_FEW(16, 5, 6, false, 1);
+    case FEW_32: if (gated) TLLM_FEW(32, 4, 5, true, 1); else TLLM_FEW(32, 4, 5, false, 1);
+    case FEW_64: if (gated) TLLM_FEW(64, 3, 5, true, 2); else TLLM_FEW(64, 3, 4, false, 2);
+    case FEW_128: TLLM_FEW(128, 4, 6, false, 4);
+    case TILES_128: TLLM_TILES(128, 6, false);
+    case TILES_256: if (gated) TLLM_TILES(256, 4, true); else TLLM_TILES(256, 4, false);
   }
-  if (fits(16, 1)) TLLM_FEW(16, 5, 6, false, 1);
-  if (fits(32, 2)) TLLM_FEW(32, 4, 5, false, 1);
-  if (m <= 64 && w_tiles <= 65535) TLLM_FEW(64, 3, 4, false, 2);
-  if (((m + 127) / 128) * w_tiles <= 74) TLLM_FEW(128, 4, 6, false, 4);
-  if (((m + 127) / 128) * (long long)((n + 255) / 256) >= 74) TLLM_TILES(256, 4, false);
-  TLLM_TILES(128, 6, false);
 #undef TLLM_FEW
 #undef TLLM_TILES
+  return TLLM_ERR_ARG;
+}
+// Which kernel a product of these sizes runs on, as Kernel numbers them, and into how many slices it cuts K on the current device: what the tests
+// that name a kernel ask.
+extern "C" int tllm_linear_fp8_kernel(int m, int n, int k, int gated, int* slices) {
+  Fp8Args p = {};
+  p.m = m; p.n = n; p.k = k; p.w_rows = gated ? 256 * ((n + 127) / 128) : n; p.groups = (k + BK - 1) / BK;
+  const Kernel kernel = pick_kernel(p, gated);
+  *slices = kernel == FEW_16 ? (gated ? pick_slices<16, 2, true, 1, 24>(p) : pick_slices<16, 5, false, 1, 24>(p))
+          : kernel == FEW_32 ? (gated ? pick_slices<32, 4, true, 1, 40>(p) : pick_slices<32, 4, false, 1, 40>(p))
+          : kernel == FEW_64 ? (gated ? pick_slices<64, 3, true, 2, 72>(p) : pick_slices<64, 3, false, 2, 72>(p))
+          : kernel == FEW_128 ? pick_slices<128, 4, false, 4, 136>(p) : 1;
+  return kernel;
 }
