@@ -825,20 +825,25 @@ static int launch_few(const Fp8Args& p, const FewArgs& f, const void* a, long lo
 }
 
 // How many clusters of `slices` CTAs the current device runs side by side: a cluster stays within a group of SMs, so that sizes that do
-// not divide the group leave some of its SMs idle (with a CTA per SM, 74 of two, 45 of three, 33, 26, 22, 15, 15).  Asked once per kernel,
-// size and device.  The answer counts one CTA per SM for kernels that use tensor memory, of which RESIDENT run (296 CTAs of 128 values of
-// K take 3.0 us, 297 4.4).
+// not divide the group leave some of its SMs idle.  `alone`: with a CTA per SM (74 of two, 45 of three, 33, 26, 22, 15, 15; what the runtime
+// answers for kernels that use tensor memory, however many of them fit an SM); `all`: with the RESIDENT ones that do run (two: 148, 93, 71, 56,
+// 45, 37, 33; 296 CTAs of 128 values of K take 3.0 us, 297 4.4), which the runtime is asked about a kernel of the same size that does not.
+// Asked once per kernel, size and device.
+struct Clusters { int alone, all; };
+template <int THREADS, int RESIDENT>
+__global__ void __launch_bounds__(THREADS, RESIDENT) places_kernel() {}      // (never launched)
 template <int BN, int STAGES, bool GATED, int HALVES, int SENT>
-static int most_clusters(int slices) {
+static Clusters most_clusters(int slices) {
   using L = FewSmem<BN, STAGES, GATED, HALVES, true, SENT>;
   static std::atomic<int> held[PerDeviceLimit::DEVICES][9] = {};
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= PerDeviceLimit::DEVICES) return 0;
-  int n = held[dev][slices].load(std::memory_order_relaxed);
-  if (n > 0) return n - 1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= PerDeviceLimit::DEVICES) return {0, 0};
+  const int known = held[dev][slices].load(std::memory_order_relaxed);
+  if (known > 0) return {known >> 16, (known & 0xFFFF) - 1};
   auto kern = linear_fp8_few_kernel<BN, STAGES, GATED, HALVES, true, SENT>;
-  static PerDeviceLimit limit;
-  if (reserve_smem(limit, L::TOTAL, kern) != cudaSuccess) return 0;
+  auto places = places_kernel<L::THREADS, L::RESIDENT>;
+  static PerDeviceLimit limit, places_limit;
+  if (reserve_smem(limit, L::TOTAL, kern) != cudaSuccess || reserve_smem(places_limit, L::TOTAL, places) != cudaSuccess) return {0, 0};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(1, 1, slices);
   cfg.blockDim = dim3(L::THREADS);
@@ -850,22 +855,24 @@ static int most_clusters(int slices) {
   attr[0].val.clusterDim.z = slices;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) return 0;
-  n *= L::RESIDENT;
-  held[dev][slices].store(n + 1, std::memory_order_relaxed);
+  Clusters n = {};
+  if (cudaOccupancyMaxActiveClusters(&n.alone, kern, &cfg) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n.all, places, &cfg) != cudaSuccess) return {0, 0};
+  held[dev][slices].store((n.alone << 16) + n.all + 1, std::memory_order_relaxed);
   return n;
 }
 
 // Slices of K: as many as leave four groups to each, eight at most, and let all tiles run at once (6,144 x 4,096, 48 tiles: 6 slices in
-// two rounds 9.5 us, 5 in one 6.6; 2,560 x 2,048: 8 slices of two groups 4.0, 4 of four 3.8).  Where the slices are long, a few clusters
-// more than run at once cost less than fewer slices (4,096 x 14,336, 32 tiles: 8 slices of 14 groups, 30 clusters at once, 11.0 us, 6 of
-// 19 12.1).
+// two rounds 9.5 us, 5 in one 6.6; 2,560 x 2,048: 8 slices of two groups 4.0, 4 of four 3.8).  Places where a cluster of one SM group's
+// last CTAs shares SMs with its others are counted where the slices have twelve groups or more (8 rows, us without / with them: 4,096 columns, 32
+// tiles on 33 places instead of 30, 8 slices of 4 groups 4.7 / 4.9, of 8 7.6 / 7.0, of 12 10.7 / 9.4, of 20 15.1 / 13.6; 8,960 columns, 70 on
+// 71 instead of 66, 4 slices of 4 4.9 / 5.1, of 8 8.0 / 7.4, of 12 11.0 / 9.8; 7,040, 55 on 56 instead of 52, 5 slices of 8 7.7 / 8.1, of
+// 12 10.4 / 10.6, of 64 rows 13.7 / 12.8).  Beyond them a second round begins (5,888, 46 on 45, 6 slices of 12: 10.4 / 14.8).
 template <int BN, int STAGES, bool GATED, int HALVES, int SENT>
 static int pick_slices(const Fp8Args& p) {
   const long long tiles = ((p.n + 127) / 128) * (long long)((p.m + BN - 1) / BN);
   for (int slices = min(8, p.groups / 4); slices > 1; --slices) {
-    const int most = most_clusters<BN, STAGES, GATED, HALVES, SENT>(slices);
-    if (tiles <= (p.groups >= 12 * slices ? most + most / 15 : most)) return slices;
+    const Clusters most = most_clusters<BN, STAGES, GATED, HALVES, SENT>(slices);
+    if (tiles <= (p.groups >= 12 * slices ? most.all : most.alone * FewSmem<BN, STAGES, GATED, HALVES, true, SENT>::RESIDENT)) return slices;
   }
   return 1;
 }
