@@ -645,3 +645,10 @@ def test_slices_of_one_round(ops):
     if torch.cuda.get_device_properties(0).multi_processor_count == 148:
         assert all(s * tiles <= 2 * 148 for tiles, s in enumerate(by_tiles, 1) if s > 1)
         assert cut(8, 46 * 128, 9216) < 6 and cut(8, 92 * 128, 4608) <= 3 and cut(8, 157 * 128, 5120) == 1
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k", [(300, 14336), (4000, 1030), (1481, 2550), (1400, 1000), (1200, 4096)])
+def test_rows_of_long_runs(ops, m, k, dtype):
+    """More groups than the kernel of short runs takes (12,432 of float32, 29,600 of bfloat16), and next to them."""
+    test_rows_are_the_nearest_8_bit_values(ops, m, k, dtype)

@@ -62,9 +62,12 @@ constexpr int ROWS_THREADS = 256;
 // A warp per row and run of groups, all of the run's loads in flight together: four groups of float32, four values per lane, or
 // eight of bfloat16, eight values per lane and half a warp per group.  With 16-byte loads and no checks inside a run the kernel
 // issues 25 instructions per group of bfloat16 instead of 86 and is bound by memory.
-// (Few rows: runs a quarter as long, so that four times the warps share the work.)
-template <typename T> struct Run { static constexpr int LONG = 4, SHORT = 1; };
-template <> struct Run<__nv_bfloat16> { static constexpr int LONG = 8, SHORT = 2; };
+// Few groups: runs a quarter as long, so that four times the warps share the work.  us, long / short, by groups in all:
+//   bfloat16  4,700 1.7 / 1.4 and 4.4 / 2.6 (rows of 2,048 and 1,000), 11,000 3.4 / 2.3, 16,500 3.8 / 2.3, 18,944 2.2 / 2.4, 22,000 3.7 / 2.6, 30,000 3.9 / 3.3,
+//             40,000 4.0 / 4.0
+//   float32   4,700 2.9 / 1.8, 9,500 2.0 / 2.3 and 2.4 / 2.2, 11,000 2.8 / 2.4, 12,500 2.7 / 2.6, 14,200 2.1 / 2.8, 16,500 2.9 / 3.1, 22,000 3.0 / 3.9
+template <typename T> struct Run { static constexpr int LONG = 4, SHORT = 1, FEW = 148 * 84; };
+template <> struct Run<__nv_bfloat16> { static constexpr int LONG = 8, SHORT = 2, FEW = 148 * 200; };
 
 template <typename T, int GROUPS>
 __global__ void __launch_bounds__(ROWS_THREADS)
@@ -304,7 +307,7 @@ extern "C" int tllm_quantize_fp8(const QuantizeCall* c) {
   const auto [x, ldx, out, ldo, scales, lds, rows, width, dtype, stream] = *c;
   if (int e = check_rows("quantize_fp8", rows, width, out, ldo, lds)) return e;
   const int groups = (width + FP8_GROUP - 1) / FP8_GROUP;
-  const bool few = (long long)rows * groups <= 148 * 32;     // (33 rows of 2,000: short runs 1.7 us, long ones 3.5)
+  const bool few = (long long)rows * groups <= (dtype == TLLM_F32 ? Run<float>::FEW : Run<__nv_bfloat16>::FEW);
   const int run = dtype == TLLM_F32 ? (few ? Run<float>::SHORT : Run<float>::LONG) : (few ? Run<__nv_bfloat16>::SHORT : Run<__nv_bfloat16>::LONG);
   const int runs = (groups + run - 1) / run;
   TLLM_REQUIRE((long long)rows * runs < (1ll << 31), "quantize_fp8: %d rows of %d values are too many for one launch", rows, width);
