@@ -652,3 +652,9 @@ def test_slices_of_one_round(ops):
 def test_rows_of_long_runs(ops, m, k, dtype):
     """More groups than the kernel of short runs takes (12,432 of float32, 29,600 of bfloat16), and next to them."""
     test_rows_are_the_nearest_8_bit_values(ops, m, k, dtype)
+
+
+@pytest.mark.parametrize("m,k", [(3700, 520), (2368, 1000), (2367, 1030), (1184, 2048), (1200, 2050), (600, 4096), (640, 4101), (297, 8192), (330, 8000), (9, 9000), (200, 14336)])
+def test_normed_rows_of_few_and_many_groups(ops, m, k):
+    """Next to 18,944 groups in all, where a warp gets eight of them instead of one, two or four, and rows of more than 64 groups."""
+    test_normed_rows(ops, m, k)

@@ -334,9 +334,12 @@ extern "C" int tllm_rms_norm_fp8(const RmsNormCall* c) {
   if (int e = check_rows("rms_norm_fp8", rows, width, out, ldo, lds)) return e;
   const int groups = (width + FP8_GROUP - 1) / FP8_GROUP;
   const int vec = (uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0 && width % 4 == 0;
-  // Few rows leave most SMs idle: a warp per group is the shortest way through a row.  Many rows: eight groups per warp, so that more
-  // rows fit an SM.
-  const int per = rows <= 296 ? (groups <= 16 ? 1 : groups <= 32 ? 2 : groups <= 64 ? 4 : 8) : 8;
+  // Few groups in all leave SMs idle: a warp per group is the shortest way through a row, up to 16 groups; more of them per warp where the row has
+  // more.  Many groups: eight per warp, so that more rows fit an SM.  us, eight / fewer, by rows x values (groups in all):
+  //   592 x 1,000 (4,736) 3.0 / 2.0, 320 x 2,048 (5,120) 4.1 / 2.5, 444 x 4,096 (14,208) 4.5 / 2.9, 592 x 4,096 (18,944) 4.6 / 3.8, 296 x 8,192
+  //   (18,944) 4.1 / 3.3, 1,184 x 2,048 (18,944) 4.5 / 4.5, 320 x 8,192 (20,480) 4.1 / 4.5, 812 x 4,096 (25,984) 4.6 / 4.9, 1,625 x 2,048 (26,000) 4.6 / 5.7
+  const bool few = (long long)rows * groups <= 148 * 128;
+  const int per = !few ? 8 : groups <= 16 ? 1 : groups <= 32 ? 2 : groups <= 64 ? 4 : 8;
   const int warps = min(32, max(1, (groups + per - 1) / per));
   const bool full = vec && width % FP8_GROUP == 0;
   auto pick = [&](auto whole) {
