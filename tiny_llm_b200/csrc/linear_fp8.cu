@@ -750,13 +750,14 @@ linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   };
   bool met = false;
   for (int i = here ? warp : own_tokens; i < own_tokens; i += WARPS) met = leave(i, std::false_type()) || met;
-  if (__builtin_expect(__any_sync(0xffffffffu, met), 0))
-    for (int i = warp; i < own_tokens; i += WARPS) leave(i, std::true_type());
   // Everybody has sent (whoever has its sums knows that already).  A CTA that gave up waiting for them stays until they have landed.
   if (SLICED) {
     cluster_wait();
     if (!here) mbar_drain(sums_bar, 1, 1);
   }
+  // (Last of all, so that the others end without a jump over it: 64 x 5,632 x 2,048 gated 10.8 us where it stood before the cluster's barrier.)
+  if (!__any_sync(0xffffffffu, met)) return;
+  for (int i = warp; i < own_tokens; i += WARPS) leave(i, std::true_type());
 }
 
 // ---------------------------------------------------------------- host side
