@@ -658,3 +658,38 @@ def test_rows_of_long_runs(ops, m, k, dtype):
 def test_normed_rows_of_few_and_many_groups(ops, m, k):
     """Next to 18,944 groups in all, where a warp gets eight of them instead of one, two or four, and rows of more than 64 groups."""
     test_normed_rows(ops, m, k)
+
+
+def test_the_first_calls_of_a_process_may_be_captured():
+    """Loading, limits and what the runtime is asked happen inside the capture then."""
+    import os
+    import subprocess
+    import sys
+    script = """
+import torch
+from tiny_llm_b200 import ops
+g = torch.Generator(device="cuda").manual_seed(0)
+x, w = (torch.randn(*s, generator=g, device="cuda") for s in ((700, 640), (4096, 640)))
+norm, out, few = torch.ones(640, device="cuda"), torch.zeros(700, 4096, device="cuda"), torch.zeros(3, 4096, device="cuda")
+a, b, q, h = ops.fp8_rows(700, 640, "cuda"), ops.fp8_rows(700, 640, "cuda"), ops.fp8_weight(4096, 640, "cuda"), ops.fp8_rows(700, 2048, "cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    ops.quantize_weight_fp8(w, *q)
+    ops.rms_norm_fp8(x, norm, 1e-5, *b)
+    ops.quantize_fp8(x, *a)
+    ops.linear_swiglu_fp8(*b, *q, *h)
+    ops.linear_fp8(*a, *q, out)
+    ops.linear_fp8(a[0][:3], a[1][:3], *q, few)
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in (out, few, h[0].float(), h[1].float())]
+ops.linear_fp8(*a, *q, out)
+ops.linear_fp8(a[0][:3], a[1][:3], *q, few)
+ops.linear_swiglu_fp8(*b, *q, *h)
+assert all(torch.equal(x, y) for x, y in zip(got, (out, few, h[0].float(), h[1].float()))) and float(out.norm()) > 0 and float(few.norm()) > 0
+ops.check_status()
+print("the same")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, cwd=root, timeout=300)
+    assert r.returncode == 0 and r.stdout.split("\n")[-2] == "the same", r.stderr

@@ -52,7 +52,7 @@ static Gate make_gate(int act, float limit) {
   return {-inf, inf, inf, 1.f, 0.f, 0.f, 0.f};
 }
 struct Fp8Args {
-  const uint8_t *a, *w;        // e4m3 rows, for far_sum (the products read them through the copy unit)
+  const uint8_t *a, *w;        // e4m3 rows, for the sums made once more (the products read them through the copy unit)
   const uint8_t* a_scales;     // [m][lda_s] e8m0
   const float* w_scales;       // [ceil(n / 128)][groups]
   void* out;
@@ -85,9 +85,10 @@ __device__ __forceinline__ float gate_f(float g, float u, const Gate& q) {
 // A group's sum meets the product of two scales, which may lie anywhere in 32 bits: the product may leave them although the result does not
 // (2^100 * 2^40 beside a sum of 0 or 2^-18), or keep few bits below 2^-126.  The kernels note such products, and the elements they belong to are
 // summed once more, one by one and in 64 bits.  The scales of a model's rows and weights lie within a few powers of ten, so this is for
-// being right and not for speed: a row of 14,336 values takes milliseconds, of some millions longer than the other warps wait, which the
-// status word then says.  The way of all others pays an instruction or two per product for it (1 x 2,560 x 2,048 3.08 us -> 3.13, gated
-// 8 x 5,632 x 2,048 5.74 -> 5.82, many rows nothing).  Two factors in place of the product, applied one after the other, cost every call 2 to 7 %.
+// being right and not for speed: with such a product in each row, 8 rows of 4,096 x 14,336 take 6 ms and 2,048 rows 70 (20 per tile; the
+// CTA's other warps wait for 2 s, which a K of a million and a half would use up, as the status word then says).  The way of all others
+// pays an instruction or two per product for it (1 x 2,560 x 2,048 3.08 us -> 3.12, 64 x 5,632 x 2,048 gated 10.3 -> 10.6, many rows at most
+// 2 %).  Two factors in place of the product, applied one after the other, cost every call 2 to 7 %.
 __device__ __forceinline__ uint32_t far_key(float s) { return 2u * __float_as_uint(s) - 0x01000000u; }      // FAR or more unless s is a normal number
 constexpr uint32_t FAR = 0xFE000000u;
 // (zeros, infinities and NaN among the scales themselves give what they give)
@@ -105,6 +106,49 @@ __device__ __forceinline__ float far_sum(const Fp8Args& p, int m, int w_row) {
     sum += part * fp8_scale(sa[g]) * sw[g];
   }
   return (float)sum;
+}
+
+// sixteen values of a row from `k` on, zeros behind its last
+__device__ __forceinline__ void load16(const uint8_t* row, int k, int width, float* v) {
+  uint4 u = make_uint4(0u, 0u, 0u, 0u);
+  if (k + 16 <= width) {
+    u = *reinterpret_cast<const uint4*>(row + k);
+  } else {
+    for (int e = 0; k + e < width; ++e) (&u.x)[e / 4] |= (uint32_t)row[k + e] << (8 * (e % 4));
+  }
+#pragma unroll
+  for (int e = 0; e < 16; e += 2) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((&u.x)[e / 4] >> (8 * (e % 4))), __NV_E4M3);
+    const float2 f = __half22float2(__half2(h));
+    v[e] = f.x; v[e + 1] = f.y;
+  }
+}
+// The same for 32 neighbouring rows of the weight, 0 behind the last one (what a thread of the large tiles has): sixteen products at a time in 32
+// bits, five roundings each at most, scaled and added up in 64.
+__device__ __noinline__ void far_sums(const Fp8Args& p, int m, int w_row, float* again) {
+  double sums[32];
+#pragma unroll 1
+  for (int j = 0; j < 32; ++j) sums[j] = 0.;
+  const uint8_t *a = p.a + m * p.lda, *sa = p.a_scales + m * p.lda_s;
+#pragma unroll 1
+  for (int k = 0; k < p.k; k += 16) {
+    const int g = k / BK;
+    const double scale = fp8_scale(sa[g]);
+    float x[16];
+    load16(a, k, p.k, x);
+#pragma unroll 1
+    for (int j = 0; j < 32; ++j) {
+      const int row = w_row + j;
+      if (row >= p.w_rows) break;
+      float y[16], part[4] = {0.f, 0.f, 0.f, 0.f};
+      load16(p.w + row * p.ldw, k, p.k, y);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) part[e % 4] = fmaf(x[e], y[e], part[e % 4]);
+      sums[j] += (double)((part[0] + part[1]) + (part[2] + part[3])) * (scale * p.w_scales[(long long)(row / 128) * p.groups + g]);
+    }
+  }
+#pragma unroll 1
+  for (int j = 0; j < 32; ++j) again[j] = (float)sums[j];
 }
 
 // e4m3 x e4m3 -> float32, M = m, N = n, both operands K-major (bits 7-9 and 10-12: 0 is e4m3)
@@ -393,16 +437,16 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         bool far = false;
         if (farthest >= FAR && m < p.m)
           for (int g = 0; g < p.groups; ++g) far = far || is_far(sa[g], sw[g]) || (GATED && is_far(sa[g], sw[p.groups + g]));
-        if (far) {
-          float again[COLS];
-#pragma unroll 1
-          for (int j = 0; j < COLS; ++j) {
-            const int w_row = tile_n * BN + column(j / 32) + j % 32;
-            again[j] = w_row < p.w_rows ? far_sum(p, m, w_row) : 0.f;
-          }
+        // (all sums pass through memory, so that none is held in a register over the calls: held, they cost the loop above a quarter)
+        float again[COLS];
 #pragma unroll
-          for (int j = 0; j < COLS; ++j) acc[j] = again[j];
+        for (int j = 0; j < COLS; ++j) again[j] = acc[j];
+        if (far) {
+#pragma unroll 1
+          for (int c = 0; c < CHUNKS; ++c) far_sums(p, m, tile_n * BN + column(c), again + 32 * c);
         }
+#pragma unroll
+        for (int j = 0; j < COLS; ++j) acc[j] = again[j];
         __syncwarp();
       }
       if (!GATED) {
