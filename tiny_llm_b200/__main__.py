@@ -30,7 +30,7 @@ FLAGS = {
     "top_p": (float, 0.95, "Sample from the smallest set of tokens whose cumulative probability > p"),
     "page_mode": (bool, True, "Paged attention (always on; accepted for compatibility)"),
     "dtype": (str, "bfloat16", "bfloat16 (serving kernels) or float32 (everything in true 32-bit)"),
-    "weights": (str, "", "fp8: the layers' matrices in 8 bits (bfloat16 engine); empty: as --dtype says"),
+    "weights": (str, "", "fp8: the layers' matrices in 8 bits (bfloat16 engine; for large models, small ones gain nothing); empty: as --dtype says"),
     "seed": (int, 0, "Seed of the sampler's random stream"),
     "page_size": (int, 16, "Tokens per cache page"),
     "max_tokens": (int, 0, "Tokens the cache pool holds (0: max_requests x the model's positions)"),

@@ -33,7 +33,9 @@ class Pipeline:
         pool holds if that is less).  `chunk`: the largest portion of one prompt in one step (default: the step's whole
         token budget; measured at the TinyLlama sizes a step of 512 prompt tokens runs at 233,000 tokens a second and a
         step of 2,048 at 448,000, so a prompt is cut no finer than the budget asks).  `weights`="fp8": the layers' matrices in 8 bits, for the
-        bfloat16 engine and models whose parts have an 8-bit form (the Llama decoder)."""
+        bfloat16 engine and models whose parts have an 8-bit form (the Llama decoder).  Measured at Llama-3-8B sizes (8 layers) one request
+        0.86 -> 0.62 ms a step, a prompt of 2,048 6.9 -> 5.6; at TinyLlama sizes 0.69 -> 0.68, 4.6 -> 4.5, and slower with 64 requests
+        (1.18 -> 1.22) and for a prompt of 512 (1.90 -> 2.13)."""
         if not chunk:
             chunk = max_tokens_per_step
         if not torch.cuda.is_available():

@@ -1720,7 +1720,9 @@ def linear_fp8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scale
                accumulate: bool = False) -> None:
     """out = a . w^T of 8-bit operands (a e4m3 [M, K] with e8m0 scales [M, ceil(K / 128)], w e4m3 [N, K] with float32 scales
     [ceil(N / 128), ceil(K / 128)] of any value), summed in 32 bits on the tensor cores and rounded once to `out` (bfloat16 or
-    float32); accumulate=True adds the product into a float32 `out`.  Any M, N and K; rows of a and w start on 16 bytes.
+    float32); accumulate=True adds the product into a float32 `out`.  Any M, N and K up to 2^31 - 4,096; rows of a and w start on 16
+    bytes.  Where the product of a row's and a block's scale is no normal float32 number, the element is summed once more in 64 bits: right,
+    but some hundred times slower.
     `w` and its scales are taken for a loaded weight (see `linear`): `quantize_weight_fp8` may come right before, but no
     other launch of this package that still runs may be writing them."""
     global launches
